@@ -30,11 +30,14 @@ EXPORTS = ["gann_open", "gann_open_device", "gann_search", "gann_search_device",
            "gann_index_info", "gann_probe_lut", "gann_probe_entry", "gann_pivot_sample", "gann_set_option",
            "gann_search_noalloc", "gann_part_export", "gann_part_attach", "gann_hop_begin", "gann_hop_requests",
            "gann_hop_step", "gann_hop_finish", "gann_hop_free", "gann_read_pages", "gann_exact_knn",
-           "gann_robust_prune", "gann_sort_unique_rows"]
+           "gann_robust_prune", "gann_sort_unique_rows", "gann_quantize_rows", "gann_matmul_i8",
+           "gann_beam_select_workspace", "gann_beam_select", "gann_reorder_states"]
 GANN_OPT_ADC_MODE, GANN_OPT_PIVOT_WARPS, GANN_OPT_NEIGHBOUR_CODES = 1, 2, 3
 LAYOUT_AUTO, LAYOUT_SEPARATE, LAYOUT_NEIGHBOUR_CODES = 0, 1, 2
 ADC_AUTO, ADC_TABLE, ADC_PIVOT, ADC_FILTERED = 0, 1, 2, 3
 METRIC_L2, METRIC_IP = 0, 1
+F32, F16, BF16 = 1, 2, 3   # gann_float
+MAX_BEAMS = 128            # beams of a group, and candidates kept
 
 
 class GustANNError(RuntimeError):
@@ -72,6 +75,12 @@ class _Info(C.Structure):
                 ("nav_start", C.c_int32), ("device_bytes", C.c_int64)]
 
 
+class _State(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("src_group", C.c_int64), ("src_beam", C.c_int64),
+                ("src_stride", C.c_int64 * 2), ("dst_group", C.c_int64), ("dst_beam", C.c_int64),
+                ("dst_stride", C.c_int64 * 2), ("size", C.c_int64 * 2), ("row_bytes", C.c_int64)]
+
+
 def _load() -> C.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(f"{LIB_PATH} is not built; run `python -m gustann_b200.build`")
@@ -100,6 +109,12 @@ def _load() -> C.CDLL:
     lib.gann_exact_knn.argtypes = [vp, i64, i64, i32, i32, vp, i64, i64, i32, i32, vp, vp, i32, vp]
     lib.gann_robust_prune.argtypes = [vp, i64, i64, i32, i32, vp, i64, vp, vp, i32, i32, C.c_float, vp, vp, i32, vp]
     lib.gann_sort_unique_rows.argtypes = [vp, vp, i64, i32, vp, vp, i32, vp]
+    lib.gann_quantize_rows.argtypes = [vp, i64, i64, i32, i32, vp, i64, vp, i32, vp]
+    lib.gann_matmul_i8.argtypes = [vp, i64, i64, vp, vp, i64, i64, vp, vp, i32, vp, i64, i32, i32, vp]
+    lib.gann_beam_select_workspace.argtypes = [i64, i32, i32, i32, i32, C.POINTER(i64)]
+    lib.gann_beam_select.argtypes = [vp, i32, i64, i64, vp, vp, i64, i32, i32, i32, i32, i32, vp, vp, vp, vp, i64,
+                                     i32, vp]
+    lib.gann_reorder_states.argtypes = [C.POINTER(_State), i32, vp, i64, i32, i32, i32, vp]
     for name in EXPORTS:
         if name != "gann_last_error":
             getattr(lib, name).restype = C.c_int
@@ -432,6 +447,279 @@ def sort_unique_rows(ids, dists, stream: int = 0):
     _check(lib.gann_sort_unique_rows(i.data_ptr(), d.data_ptr(), rows, k, oi.data_ptr(), od.data_ptr(),
                                      i.device.index or 0, stream or None))
     return oi, od
+
+
+def _fail(msg: str):
+    raise GustANNError(GANN_EINVAL, msg)
+
+
+def _float_code(dtype, who: str) -> int:
+    import torch
+    code = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(dtype)
+    if code is None:
+        _fail(f"{who}: dtype must be float32, float16 or bfloat16")
+    return code
+
+
+def _on_cuda(who: str, *tensors):
+    dev = tensors[0].device
+    for t in tensors:
+        if not t.is_cuda or t.device != dev:
+            _fail(f"{who}: tensors must be on one CUDA device")
+    return dev
+
+
+class _Stream:
+    """Outputs and workspaces of a call are allocated on the stream it runs on:
+    ``stream`` (a ``cudaStream_t``; 0 the default stream), or torch's current
+    stream of the device when it is None."""
+
+    def __init__(self, device, stream):
+        import torch
+        cur = torch.cuda.current_stream(device).cuda_stream
+        self.handle = cur if stream is None else stream
+        self._ctx = None
+        if self.handle != cur:
+            self._ctx = torch.cuda.stream(torch.cuda.ExternalStream(stream, device) if stream
+                                          else torch.cuda.default_stream(device))
+
+    def __enter__(self):
+        if self._ctx is not None:
+            self._ctx.__enter__()
+        return self.handle or None
+
+    def __exit__(self, *exc):
+        if self._ctx is not None:
+            self._ctx.__exit__(*exc)
+
+
+def _extent(t):
+    """First byte of a tensor and the byte behind its last one."""
+    span = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+    return t.data_ptr(), t.data_ptr() + span * t.element_size()
+
+
+def _disjoint(a, b) -> bool:
+    (a0, a1), (b0, b1) = _extent(a), _extent(b)
+    return a1 <= b0 or b1 <= a0
+
+
+def quantize_rows(x, stream: int | None = None):
+    """Rows of ``x`` [n, d] (float32, float16 or bfloat16 CUDA tensor, contiguous
+    rows) as 8-bit codes with one scale each (``gann_quantize_rows``): ``scale =
+    max|x| / 127``, ``code = x / scale`` to the nearest integer. Returns ``(codes
+    int8 [n, d], scales float32 [n])``; the codes' rows start on 16-byte
+    boundaries, as :func:`matmul_i8` wants them. A row with a NaN or an
+    infinity gets scale NaN and codes 0. ``stream``: a ``cudaStream_t``, or
+    None for torch's current stream."""
+    import torch
+    if x.dim() != 2:
+        _fail("quantize_rows: x must have two dimensions")
+    dt = _float_code(x.dtype, "quantize_rows")
+    dev = _on_cuda("quantize_rows", x)
+    n, d = x.shape
+    if d > 1 and x.stride(1) != 1:
+        _fail("quantize_rows: rows must be contiguous")
+    with _Stream(dev, stream) as st:
+        codes = torch.empty((n, (d + 15) // 16 * 16), dtype=torch.int8, device=dev)
+        scales = torch.empty(n, dtype=torch.float32, device=dev)
+        _check(lib.gann_quantize_rows(x.data_ptr(), n, x.stride(0) * x.element_size(), d, dt, codes.data_ptr(),
+                                      codes.stride(0), scales.data_ptr(), dev.index or 0, st))
+    return codes[:, :d], scales
+
+
+def _i8_rows(name: str, codes, scales):
+    import torch
+    if codes.dtype != torch.int8 or codes.dim() != 2:
+        _fail(f"matmul_i8: {name} must be int8 with two dimensions")
+    n, k = codes.shape
+    if scales.dtype != torch.float32 or scales.shape != (n,) or (n > 1 and scales.stride(0) != 1):
+        _fail(f"matmul_i8: {name}'s scales must be contiguous float32, one a row")
+    if k > 1 and codes.stride(1) != 1:
+        _fail(f"matmul_i8: rows of {name} must be contiguous")
+    stride = codes.stride(0) if n > 1 else (k + 15) // 16 * 16
+    if n and (stride % 16 or codes.data_ptr() % 16):
+        _fail(f"matmul_i8: rows of {name} must start on 16-byte boundaries, as quantize_rows lays them out")
+    return n, k, stride
+
+
+def matmul_i8(a, a_scales, b, b_scales, bias=None, dtype=None, out=None, stream: int | None = None):
+    """``out[i, j] = (a[i] . b[j]) * a_scales[i] * b_scales[j] + bias[j]`` of 8-bit
+    rows (``gann_matmul_i8``): ``a`` [m, k] and ``b`` [n, k] int8 CUDA tensors
+    whose rows start on 16-byte boundaries (:func:`quantize_rows` makes them),
+    scales float32 [m] and [n], ``bias`` float32 [n] or None. Sums are exact.
+    Returns ``out`` [m, n] of ``dtype`` (float32 unless given; float16 and
+    bfloat16 too), or fills ``out`` when it is given (contiguous rows).
+    Queries against base rows: their scores; tokens against the rows of a
+    weight matrix: a linear layer. ``stream`` as in :func:`quantize_rows`."""
+    import torch
+    m, k, sa = _i8_rows("a", a, a_scales)
+    n, kb, sb = _i8_rows("b", b, b_scales)
+    if k != kb:
+        _fail("matmul_i8: a and b must have the same number of columns")
+    ins = [a, a_scales, b, b_scales]
+    if bias is not None:
+        if bias.dtype != torch.float32 or bias.shape != (n,) or (n > 1 and bias.stride(0) != 1):
+            _fail("matmul_i8: bias must be contiguous float32, one a row of b")
+        ins.append(bias)
+    dev = _on_cuda("matmul_i8", *ins)
+    if out is not None:
+        _on_cuda("matmul_i8", a, out)
+        if out.shape != (m, n) or (dtype is not None and out.dtype != dtype):
+            _fail("matmul_i8: out must be [m, n] of the given dtype")
+        if (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
+            _fail("matmul_i8: rows of out must be contiguous and apart from each other")
+        if not all(_disjoint(out, t) for t in ins):
+            _fail("matmul_i8: out overlaps an input")
+    dt = _float_code(out.dtype if out is not None else dtype or torch.float32, "matmul_i8")
+    with _Stream(dev, stream) as st:
+        if out is None:
+            out = torch.empty((m, n), dtype=dtype or torch.float32, device=dev)
+        _check(lib.gann_matmul_i8(a.data_ptr(), m, sa, a_scales.data_ptr(), b.data_ptr(), n, sb, b_scales.data_ptr(),
+                                  None if bias is None else bias.data_ptr(), k, out.data_ptr(),
+                                  out.stride(0) if m > 1 else n, dt, dev.index or 0, st))
+    return out
+
+
+def beam_select(scores, logits, k: int, log_softmax: bool = False, finished=None, end_token: int = 0,
+                stream: int | None = None):
+    """The best ``k`` continuations of each group's beams (``gann_beam_select``):
+    ``scores`` [g, w] float32, ``logits`` [g, w, v] float32, float16 or bfloat16
+    (any strides with v contiguous). A candidate is worth ``scores[g, b] +
+    logits[g, b, t]``, or with ``log_softmax`` ``scores[g, b] +
+    log_softmax(logits[g, b])[t]``; the largest come first, equal ones in
+    ascending order of (b, t). Logits that are NaN or infinite are masked;
+    beams whose score is not finite are dead. ``finished`` [g, w] bool: such a
+    beam has one candidate, ``end_token`` at its own score. Returns ``(scores
+    float32, parents int32, tokens int32)``, each [g, k], filled up with
+    -inf, -1, -1. w and k at most 128. ``stream`` as in :func:`quantize_rows`."""
+    import torch
+    if logits.dim() != 3 or scores.dtype != torch.float32 or scores.shape != logits.shape[:2]:
+        _fail("beam_select: need logits [g, w, v] and float32 scores [g, w]")
+    dt = _float_code(logits.dtype, "beam_select")
+    g, w, v = logits.shape
+    ins = [scores, logits]
+    if finished is not None:
+        if finished.dtype not in (torch.bool, torch.uint8) or finished.shape != (g, w):
+            _fail("beam_select: finished must be bool [g, w]")
+        ins.append(finished)
+    dev = _on_cuda("beam_select", *ins)
+    if v > 1 and logits.stride(2) != 1:
+        _fail("beam_select: the last dimension of logits must be contiguous")
+    with _Stream(dev, stream) as st:
+        scores = scores.contiguous()
+        if finished is not None:
+            finished = finished.contiguous()
+        need = C.c_int64()
+        _check(lib.gann_beam_select_workspace(g, w, v, k, dev.index or 0, C.byref(need)))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
+        out_s = torch.empty((g, k), dtype=torch.float32, device=dev)
+        out_p = torch.empty((g, k), dtype=torch.int32, device=dev)
+        out_t = torch.empty((g, k), dtype=torch.int32, device=dev)
+        _check(lib.gann_beam_select(logits.data_ptr(), dt, logits.stride(0), logits.stride(1), scores.data_ptr(),
+                                    None if finished is None else finished.data_ptr(), g, w, v, k,
+                                    int(bool(log_softmax)), end_token, out_s.data_ptr(), out_p.data_ptr(),
+                                    out_t.data_ptr(), None if ws is None else ws.data_ptr(), need.value,
+                                    dev.index or 0, st))
+    return out_s, out_p, out_t
+
+
+def _state_layout(src, dst):
+    """The dimensions behind (group, beam) of two tensors of one shape as at most
+    two strided dimensions and a run of contiguous bytes (None if they do not
+    fit)."""
+    es = src.element_size()
+    dims = [(n, a, b) for n, a, b in zip(src.shape[2:], src.stride()[2:], dst.stride()[2:]) if n != 1]
+    run = 1
+    while dims and dims[-1][1] == run and dims[-1][2] == run:
+        run *= dims.pop()[0]
+    merged = []
+    for n, a, b in dims:
+        if merged and merged[-1][1] == n * a and merged[-1][2] == n * b:
+            merged[-1] = (merged[-1][0] * n, a, b)
+        else:
+            merged.append((n, a, b))
+    if len(merged) > 2:
+        return None
+    merged = [(1, 0, 0)] * (2 - len(merged)) + merged
+    return [m[0] for m in merged], [m[1] * es for m in merged], [m[2] * es for m in merged], run * es
+
+
+def _apart(t) -> bool:
+    """No two elements of the tensor share memory (sufficient test)."""
+    span = 1
+    for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if s < span:
+            return False
+        span = s * (n - 1) + span
+    return True
+
+
+def reorder_states(states, parents, out=None, stream: int | None = None):
+    """The states that follow the selected beams (``gann_reorder_states``):
+    ``out[g, j] = states[g, parents[g, j]]``. ``states``: a CUDA tensor [g, w, ...] of any
+    type, or a list of them, each moved; behind (g, w) its dimensions may be
+    strided as far as they are a contiguous run and two strided dimensions (a
+    slice of a cache's positions, or layers and heads). ``parents`` int32 [g, k], as
+    :func:`beam_select` returns; a parent outside [0, w) gives zeros. Without
+    ``out`` new tensors [g, k, ...] are returned; ``out`` gives the targets,
+    and may be ``states`` itself: in place (k <= w; beams from k on stay as they were).
+    Other overlaps are refused. ``stream`` as in :func:`quantize_rows`."""
+    import torch
+    one = torch.is_tensor(states)
+    srcs = [states] if one else list(states)
+    if parents.dim() != 2 or parents.dtype != torch.int32:
+        _fail("reorder_states: parents must be int32 [g, k]")
+    g, k = parents.shape
+    dev = _on_cuda("reorder_states", parents, *srcs)
+    for s in srcs:
+        if s.dim() < 2 or s.shape[0] != g or s.shape[1] != srcs[0].shape[1]:
+            _fail("reorder_states: every state must be [g, w, ...] with the groups of parents")
+    if not srcs:
+        return []
+    w = srcs[0].shape[1]
+    with _Stream(dev, stream) as st:
+        if out is None:
+            dsts = [torch.empty((g, k) + s.shape[2:], dtype=s.dtype, device=dev) for s in srcs]
+        else:
+            dsts = [out] if torch.is_tensor(out) else list(out)
+            _check_targets(srcs, dsts, parents, g, k)
+        table = (_State * len(srcs))()
+        for e, s, d in zip(table, srcs, dsts):
+            lay = _state_layout(s, d)
+            if lay is None:
+                _fail("reorder_states: a state has more than two strided dimensions behind (g, w)")
+            es = s.element_size()
+            e.src, e.dst = s.data_ptr(), d.data_ptr()
+            e.src_group, e.src_beam = s.stride(0) * es, s.stride(1) * es
+            e.dst_group, e.dst_beam = d.stride(0) * es, d.stride(1) * es
+            e.size[:], e.src_stride[:], e.dst_stride[:], e.row_bytes = lay
+        _check(lib.gann_reorder_states(table, len(srcs), parents.contiguous().data_ptr(), g, w, k, dev.index or 0, st))
+    return dsts[0] if one else dsts
+
+
+def _check_targets(srcs, dsts, parents, g, k):
+    if len(dsts) != len(srcs):
+        _fail("reorder_states: one target for each state")
+    _on_cuda("reorder_states", parents, *dsts)
+    for s, d in zip(srcs, dsts):
+        same = d.data_ptr() == s.data_ptr() and d.shape == s.shape and d.stride() == s.stride()
+        if d.dtype != s.dtype or d.shape != ((g,) + (s.shape[1] if same else k,) + s.shape[2:]):
+            _fail("reorder_states: a target must be [g, k, ...] of its state's type, or the state itself")
+        if same and k > s.shape[1]:
+            _fail("reorder_states: in place needs k <= w")
+        if not _apart(d):
+            _fail("reorder_states: elements of a target share memory")
+    # every target apart from every other array, but for its own state in place
+    spans = sorted([(*_extent(d), i, True) for i, d in enumerate(dsts)] +
+                   [(*_extent(s), i, False) for i, s in enumerate(srcs) if s.data_ptr() != dsts[i].data_ptr()] +
+                   [(*_extent(parents), -1, False)])
+    end, end_target = 0, 0
+    for a, b, _, target in spans:
+        if a < (end if target else end_target) and b > a:
+            _fail("reorder_states: a target overlaps another array")
+        end = max(end, b)
+        end_target = max(end_target, b if target else 0)
 
 
 def pivot_sample(n: int, s: int, seed: int = 114514) -> np.ndarray:

@@ -24,7 +24,8 @@ LIB = os.path.join(OUT, "libgann.so")
 CLI = os.path.join(OUT, "search_mem")
 CHECK = os.path.join(OUT, "check_recall")
 
-LIB_SOURCES = ["gann_search.cu", "gann_api.cu", "gann_loader.cpp", "gann_exact.cu", "gann_build.cu"]
+LIB_SOURCES = ["gann_search.cu", "gann_api.cu", "gann_loader.cpp", "gann_exact.cu", "gann_build.cu", "gann_quant.cu",
+               "gann_select.cu"]
 HEADERS = ["gann_internal.hpp"]
 
 

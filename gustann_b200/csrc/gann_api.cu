@@ -46,6 +46,39 @@ int dev_upload(T*& dst, const T* src, size_t count, int64_t& bytes) {
   return GANN_OK;
 }
 
+// Runs `launch(sm_count)` with `device` current and puts the caller's device back.
+template <typename F>
+int run_on_device(const char* who, int32_t device, F&& launch) {
+  int ndev = 0;
+  GANN_CUDA(cudaGetDeviceCount(&ndev));
+  if (device < 0 || device >= ndev) return set_error(GANN_EINVAL, std::string(who) + ": no such CUDA device");
+  int prev = 0, sm = 0;
+  GANN_CUDA(cudaGetDevice(&prev));
+  if (prev != device) GANN_CUDA(cudaSetDevice(device));
+  cudaError_t e = cudaDeviceGetAttribute(&sm, cudaDevAttrMultiProcessorCount, device);
+  if (e == cudaSuccess) e = launch(sm);
+  if (prev != device) cudaSetDevice(prev);
+  if (e != cudaSuccess)
+    return set_error(e == cudaErrorMemoryAllocation ? GANN_ENOMEM : GANN_ECUDA,
+                     std::string(who) + ": " + cudaGetErrorString(e));
+  return GANN_OK;
+}
+
+int64_t float_size(int32_t dtype) {
+  return dtype == GANN_F32 ? 4 : dtype == GANN_F16 || dtype == GANN_BF16 ? 2 : 0;
+}
+bool aligned_to(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+constexpr int32_t kMaxI8Dim = 131071;   // 131072 products of -128 * -128 pass 2^31 - 1
+constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1;
+
+bool select_sizes_ok(int64_t groups, int32_t beams, int32_t vocab, int32_t keep) {
+  return groups >= 0 && groups <= kMaxRows && beams >= 1 && beams <= gann::kBeamMax && keep >= 1 &&
+         keep <= gann::kBeamMax && vocab >= 1 && static_cast<int64_t>(beams) * vocab <= kMaxRows;
+}
+constexpr const char* kSelectSizes =
+    "need 0 <= groups < 2^31, 1 <= beams <= 128, 1 <= keep <= 128, vocab >= 1 and beams * vocab < 2^31";
+
 }  // namespace
 
 struct gann_handle {
@@ -1088,6 +1121,130 @@ int gann_sort_unique_rows(const int32_t* d_ids, const float* d_dists, int64_t ro
   cudaSetDevice(prev);
   if (e != cudaSuccess) return set_error(GANN_ECUDA, std::string("gann_sort_unique_rows: ") + cudaGetErrorString(e));
   return GANN_OK;
+}
+
+int gann_quantize_rows(const void* d_x, int64_t rows, int64_t x_stride, int32_t dim, int32_t dtype, int8_t* d_codes,
+                       int64_t code_stride, float* d_scales, int32_t device, void* stream) {
+  const int64_t elem = float_size(dtype);
+  if (!elem) return set_error(GANN_EINVAL, "gann_quantize_rows: dtype must be GANN_F32, GANN_F16 or GANN_BF16");
+  if (rows < 0 || rows > kMaxRows || dim < 1 || dim > kMaxI8Dim)
+    return set_error(GANN_EINVAL, "gann_quantize_rows: need 0 <= rows < 2^31 and 1 <= dim <= 131071");
+  if (x_stride < 0 || x_stride % elem || code_stride < dim || code_stride % 16)
+    return set_error(GANN_EINVAL,
+                     "gann_quantize_rows: x_stride must be a multiple of the element size, code_stride a multiple of "
+                     "16 that covers a row");
+  if (rows == 0) return GANN_OK;
+  if (!d_x || !d_codes || !d_scales || !aligned_to(d_x, elem) || !aligned_to(d_codes, 16) || !aligned_to(d_scales, 4))
+    return set_error(GANN_EINVAL, "gann_quantize_rows: null or unaligned buffer");
+  return run_on_device("gann_quantize_rows", device, [&](int sm) {
+    return gann::launch_quantize_rows(d_x, rows, x_stride, dim, dtype, d_codes, code_stride, d_scales, sm,
+                                      static_cast<cudaStream_t>(stream));
+  });
+}
+
+int gann_matmul_i8(const int8_t* d_a, int64_t m, int64_t a_stride, const float* d_a_scales, const int8_t* d_b,
+                   int64_t n, int64_t b_stride, const float* d_b_scales, const float* d_bias, int32_t k, void* d_out,
+                   int64_t out_stride, int32_t out_dtype, int32_t device, void* stream) {
+  const int64_t elem = float_size(out_dtype);
+  if (!elem) return set_error(GANN_EINVAL, "gann_matmul_i8: out_dtype must be GANN_F32, GANN_F16 or GANN_BF16");
+  if (m < 0 || m > kMaxRows || n < 0 || n > kMaxRows || k < 1 || k > kMaxI8Dim)
+    return set_error(GANN_EINVAL, "gann_matmul_i8: need 0 <= m, n < 2^31 and 1 <= k <= 131071");
+  if (a_stride < k || a_stride % 16 || b_stride < k || b_stride % 16 || out_stride < n)
+    return set_error(GANN_EINVAL,
+                     "gann_matmul_i8: a and b strides must be multiples of 16 bytes that cover a row, out_stride at "
+                     "least n");
+  if (m == 0 || n == 0) return GANN_OK;
+  if (!d_a || !d_a_scales || !d_b || !d_b_scales || !d_out || !aligned_to(d_a, 16) || !aligned_to(d_b, 16) ||
+      !aligned_to(d_a_scales, 4) || !aligned_to(d_b_scales, 4) || !aligned_to(d_bias, 4) || !aligned_to(d_out, elem))
+    return set_error(GANN_EINVAL, "gann_matmul_i8: null or unaligned buffer");
+  return run_on_device("gann_matmul_i8", device, [&](int sm) {
+    return gann::launch_matmul_i8(d_a, m, a_stride, d_a_scales, d_b, n, b_stride, d_b_scales, d_bias, k, d_out,
+                                  out_stride, out_dtype, sm, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int gann_beam_select_workspace(int64_t groups, int32_t beams, int32_t vocab, int32_t keep, int32_t device,
+                               int64_t* bytes) {
+  if (!bytes) return set_error(GANN_EINVAL, "gann_beam_select_workspace: null output");
+  if (!select_sizes_ok(groups, beams, vocab, keep))
+    return set_error(GANN_EINVAL, std::string("gann_beam_select_workspace: ") + kSelectSizes);
+  return run_on_device("gann_beam_select_workspace", device, [&](int sm) {
+    *bytes = static_cast<int64_t>(gann::beam_select_workspace(groups, beams, vocab, keep, sm));
+    return cudaSuccess;
+  });
+}
+
+int gann_beam_select(const void* d_logits, int32_t dtype, int64_t group_stride, int64_t beam_stride,
+                     const float* d_scores, const uint8_t* d_finished, int64_t groups, int32_t beams, int32_t vocab,
+                     int32_t keep, int32_t log_softmax, int32_t end_token, float* d_out_scores,
+                     int32_t* d_out_parents, int32_t* d_out_tokens, void* d_workspace, int64_t workspace_bytes,
+                     int32_t device, void* stream) {
+  const int64_t elem = float_size(dtype);
+  if (!elem) return set_error(GANN_EINVAL, "gann_beam_select: dtype must be GANN_F32, GANN_F16 or GANN_BF16");
+  if (!select_sizes_ok(groups, beams, vocab, keep))
+    return set_error(GANN_EINVAL, std::string("gann_beam_select: ") + kSelectSizes);
+  if (group_stride < 0 || beam_stride < 0) return set_error(GANN_EINVAL, "gann_beam_select: negative stride");
+  if (d_finished && (end_token < 0 || end_token >= vocab))
+    return set_error(GANN_EINVAL, "gann_beam_select: end_token must be a token when finished is given");
+  if (groups == 0) return GANN_OK;
+  if (!d_logits || !d_scores || !d_out_scores || !d_out_parents || !d_out_tokens || !aligned_to(d_logits, elem) ||
+      !aligned_to(d_scores, 4) || !aligned_to(d_out_scores, 4) || !aligned_to(d_out_parents, 4) ||
+      !aligned_to(d_out_tokens, 4))
+    return set_error(GANN_EINVAL, "gann_beam_select: null or unaligned buffer");
+  gann::SelectArgs a;
+  a.logits = d_logits;
+  a.dtype = dtype;
+  a.group_stride = group_stride;
+  a.beam_stride = beam_stride;
+  a.scores = d_scores;
+  a.finished = d_finished;
+  a.groups = groups;
+  a.beams = beams;
+  a.vocab = vocab;
+  a.keep = keep;
+  a.softmax = log_softmax != 0;
+  a.end_token = end_token;
+  a.out_scores = d_out_scores;
+  a.out_parents = d_out_parents;
+  a.out_tokens = d_out_tokens;
+  a.workspace = d_workspace;
+  bool small = false;
+  const int rc = run_on_device("gann_beam_select", device, [&](int sm) {
+    const size_t need = gann::beam_select_workspace(groups, beams, vocab, keep, sm);
+    small = need > 0 && (!d_workspace || !aligned_to(d_workspace, 16) || workspace_bytes < static_cast<int64_t>(need));
+    return small ? cudaSuccess : gann::launch_beam_select(a, sm, static_cast<cudaStream_t>(stream));
+  });
+  if (small)
+    return set_error(GANN_EINVAL, "gann_beam_select: the workspace must be 16-byte aligned and as large as "
+                                  "gann_beam_select_workspace says");
+  return rc;
+}
+
+int gann_reorder_states(const gann_state* states, int32_t count, const int32_t* d_parents, int64_t groups,
+                        int32_t beams, int32_t keep, int32_t device, void* stream) {
+  if (count < 0 || groups < 0 || groups > kMaxRows || beams < 1 || beams > gann::kBeamMax || keep < 1 ||
+      keep > gann::kBeamMax)
+    return set_error(GANN_EINVAL,
+                     "gann_reorder_states: need count >= 0, 0 <= groups < 2^31, 1 <= beams <= 128, 1 <= keep <= 128");
+  if (count == 0 || groups == 0) return GANN_OK;
+  if (!states || !d_parents || !aligned_to(d_parents, 4))
+    return set_error(GANN_EINVAL, "gann_reorder_states: null or unaligned buffer");
+  for (int32_t i = 0; i < count; ++i) {
+    const gann_state& s = states[i];
+    if (s.size[0] < 0 || s.size[1] < 0 || s.row_bytes < 0 ||
+        static_cast<__int128>(s.size[0]) * s.size[1] * s.row_bytes >= (static_cast<__int128>(1) << 62))
+      return set_error(GANN_EINVAL, "gann_reorder_states: bad size");
+    if (s.size[0] == 0 || s.size[1] == 0 || s.row_bytes == 0) continue;
+    if (!s.src || !s.dst) return set_error(GANN_EINVAL, "gann_reorder_states: null state");
+    if (s.src == s.dst &&
+        (keep > beams || s.src_group != s.dst_group || s.src_beam != s.dst_beam ||
+         s.src_stride[0] != s.dst_stride[0] || s.src_stride[1] != s.dst_stride[1]))
+      return set_error(GANN_EINVAL, "gann_reorder_states: in place needs equal strides and keep <= beams");
+  }
+  return run_on_device("gann_reorder_states", device, [&](int sm) {
+    return gann::launch_reorder_states(states, count, d_parents, groups, beams, keep, sm,
+                                       static_cast<cudaStream_t>(stream));
+  });
 }
 
 }  // extern "C"

@@ -158,6 +158,32 @@ int exact_knn_max_k();
 cudaError_t launch_exact_knn(const void* base, int64_t n, int64_t bstride, int dim, int dtype, const void* queries,
                              int64_t qstride, int64_t nq, int k, int metric, int32_t* ids, float* dists,
                              int sm_count, cudaStream_t st);
+// 8-bit rows and their products (gann_quant.cu).
+cudaError_t launch_quantize_rows(const void* x, int64_t rows, int64_t stride, int dim, int dtype, int8_t* codes,
+                                 int64_t code_stride, float* scales, int sm_count, cudaStream_t st);
+cudaError_t launch_matmul_i8(const int8_t* a, int64_t m, int64_t as, const float* sa, const int8_t* b, int64_t n,
+                             int64_t bs, const float* sb, const float* bias, int k, void* out, int64_t os, int dtype,
+                             int sm_count, cudaStream_t st);
+// Selection over beams and vocabulary, reordering of states (gann_select.cu).
+constexpr int kBeamMax = 128;     // beams of a group and candidates kept
+constexpr int kStateBatch = 32;   // state arrays of one launch
+struct SelectArgs {
+  const void* logits = nullptr;
+  int dtype = GANN_F32;
+  int64_t group_stride = 0, beam_stride = 0;   // elements
+  const float* scores = nullptr;
+  const uint8_t* finished = nullptr;           // nullable
+  int64_t groups = 0;
+  int beams = 0, vocab = 0, keep = 0, softmax = 0, end_token = 0;
+  float* out_scores = nullptr;
+  int32_t* out_parents = nullptr;
+  int32_t* out_tokens = nullptr;
+  void* workspace = nullptr;
+};
+size_t beam_select_workspace(int64_t groups, int beams, int vocab, int keep, int sm_count);
+cudaError_t launch_beam_select(const SelectArgs& a, int sm_count, cudaStream_t st);
+cudaError_t launch_reorder_states(const gann_state* states, int count, const int32_t* parents, int64_t groups,
+                                  int beams, int keep, int sm_count, cudaStream_t st);
 cudaError_t launch_gather_neighbour_codes(const uint32_t* adj, int adj_stride, int degree, const uint8_t* codes,
                                           int code_stride, int64_t n, uint8_t* out, cudaStream_t st);
 

@@ -358,6 +358,100 @@ int gann_robust_prune(const void* d_vectors, int64_t num_points, int64_t stride,
 int gann_sort_unique_rows(const int32_t* d_ids, const float* d_dists, int64_t rows, int32_t k, int32_t* d_out_ids,
                           float* d_out_dists, int32_t device, void* stream);
 
+/* Element type of float inputs and outputs of the calls below (GANN_F32 is
+ * GANN_FLOAT). */
+typedef enum { GANN_F32 = 1, GANN_F16 = 2, GANN_BF16 = 3 } gann_float;
+
+/* Rows of floats as signed 8-bit codes with one scale each, for gann_matmul_i8:
+ *   scale_i = max_j |x_ij| / 127, rounded to float32
+ *   code_ij = x_ij / scale_i rounded to the nearest integer (ties to even;
+ *             the quotient is not rounded before)
+ * so x_ij is about code_ij * scale_i, off by at most half a scale. A row of
+ * zeros has scale 0 and codes 0. A row that holds a NaN or an infinity has
+ * scale NaN and codes 0, so its products are NaN.
+ *   x       [rows x x_stride bytes] of dtype (gann_float); x_stride any
+ *           multiple of the element size, 0 repeats one row
+ *   codes   [rows x code_stride bytes]; 16-byte aligned, code_stride a multiple
+ *           of 16 and >= dim. Bytes of a row past dim are left as they were.
+ *   scales  [rows] float32
+ * Device buffers on `device`, enqueued on `stream`; inputs and outputs may not
+ * overlap. 1 <= dim <= 131071, rows < 2^31. */
+int gann_quantize_rows(const void* d_x, int64_t rows, int64_t x_stride, int32_t dim, int32_t dtype, int8_t* d_codes,
+                       int64_t code_stride, float* d_scales, int32_t device, void* stream);
+
+/* Products of 8-bit rows with a scale for each row of both sides:
+ *   out_ij = (sum_l a_il * b_jl) * a_scale_i * b_scale_j + bias_j
+ * The sum is exact (32-bit integers), then in float32: rounded, times
+ * a_scale, times b_scale plus bias in one fused step, rounded to out_dtype
+ * (values past float16's range become infinite). With a = queries and b = base
+ * rows this is their inner-product score matrix; with b_scale_j doubled and
+ * bias_j = -|x_j|^2 it ranks by squared L2; with a = tokens and b = the
+ * weights' output channels it is a linear layer.
+ *   a, b       [m x a_stride bytes], [n x b_stride bytes] int8, k columns; both
+ *              16-byte aligned, strides multiples of 16 and >= k
+ *   a_scales   [m] float32      b_scales [n] float32      bias [n] float32 or NULL
+ *   out        [m x out_stride elements] of out_dtype (gann_float),
+ *              out_stride >= n; elements of a row past n are left as they were
+ * Device buffers on `device`, enqueued on `stream`; the output may not overlap
+ * an input. 1 <= k <= 131071; m, n < 2^31. No allocation. */
+int gann_matmul_i8(const int8_t* d_a, int64_t m, int64_t a_stride, const float* d_a_scales, const int8_t* d_b,
+                   int64_t n, int64_t b_stride, const float* d_b_scales, const float* d_bias, int32_t k, void* d_out,
+                   int64_t out_stride, int32_t out_dtype, int32_t device, void* stream);
+
+/* The best `keep` continuations of each group's beams: the step of a beam
+ * search over codebook entries or tokens, and the join of several lists of
+ * scores into one. Candidate (b, t), 0 <= t < vocab, of group g is worth
+ *   scores[g][b] + logits[g][b][t]                                (log_softmax 0)
+ *   scores[g][b] + logits[g][b][t] - log sum_t exp logits[g][b][t]            (1)
+ * and the candidates are ordered by that value, largest first, compared in 64
+ * bits, equal ones by b * vocab + t. (Pass negated distances.) The sum of the
+ * exponentials is gathered in float32 and joined in 64 bits.
+ *   logits    [groups][beams][vocab] of dtype (gann_float); strides in elements
+ *             (>= 0; 0 repeats a row), vocab contiguous. NaN and infinite entries are masked:
+ *             no candidates, and not in the sum.
+ *   scores    [groups][beams] float32; a beam whose score is not finite has no
+ *             candidates
+ *   finished  [groups][beams] bytes, or NULL; a beam with a nonzero byte offers
+ *             one candidate, (b, end_token), worth scores[g][b]; its logits
+ *             are not looked at
+ *   out_scores, out_parents (b), out_tokens (t)   [groups][keep] float32, int32,
+ *             int32; slots with no candidate left are -inf, -1, -1. A value
+ *             below float32's range is written as -inf.
+ * 1 <= beams, keep <= 128; beams * vocab < 2^31; groups < 2^31.
+ * gann_beam_select_workspace gives the bytes of device memory that a call of
+ * these sizes needs (0: workspace may be NULL). The workspace needs no
+ * initialisation; calls that may overlap need one each. Device buffers on
+ * `device`, enqueued on `stream`; no allocation. */
+int gann_beam_select_workspace(int64_t groups, int32_t beams, int32_t vocab, int32_t keep, int32_t device,
+                               int64_t* bytes);
+int gann_beam_select(const void* d_logits, int32_t dtype, int64_t group_stride, int64_t beam_stride,
+                     const float* d_scores, const uint8_t* d_finished, int64_t groups, int32_t beams, int32_t vocab,
+                     int32_t keep, int32_t log_softmax, int32_t end_token, float* d_out_scores,
+                     int32_t* d_out_parents, int32_t* d_out_tokens, void* d_workspace, int64_t workspace_bytes,
+                     int32_t device, void* stream);
+
+/* One state array that follows the beams: for each group and beam a block of
+ * size[0] x size[1] rows of row_bytes contiguous bytes; all strides in bytes. */
+typedef struct {
+  const void* src;
+  void* dst;
+  int64_t src_group, src_beam, src_stride[2];
+  int64_t dst_group, dst_beam, dst_stride[2];
+  int64_t size[2];
+  int64_t row_bytes;
+} gann_state;
+
+/* dst[g][j] = src[g][parents[g][j]] for j < keep, for each of `count` state
+ * arrays (a host array of descriptors, read before the call returns). A parent
+ * outside [0, beams) gives a block of zeros. A state may be reordered in place
+ * (dst == src with the same strides, keep <= beams; beams from keep on are left
+ * as they were); other overlaps of sources and targets are not allowed.
+ *   parents  [groups][keep] int32, e.g. gann_beam_select's
+ * 1 <= beams, keep <= 128. Device buffers on `device`, enqueued on `stream`; no
+ * allocation. */
+int gann_reorder_states(const gann_state* states, int32_t count, const int32_t* d_parents, int64_t groups,
+                        int32_t beams, int32_t keep, int32_t device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
