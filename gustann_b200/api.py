@@ -507,7 +507,7 @@ def _disjoint(a, b) -> bool:
 def quantize_rows(x, stream: int | None = None):
     """Rows of ``x`` [n, d] (float32, float16 or bfloat16 CUDA tensor, contiguous
     rows) as 8-bit codes with one scale each (``gann_quantize_rows``): ``scale =
-    max|x| / 127``, ``code = x / scale`` to the nearest integer. Returns ``(codes
+    max|x| * float32(1/127)``, ``code = x / scale`` to the nearest integer. Returns ``(codes
     int8 [n, d], scales float32 [n])``; the codes' rows start on 16-byte
     boundaries, as :func:`matmul_i8` wants them. A row with a NaN or an
     infinity gets scale NaN and codes 0. ``stream``: a ``cudaStream_t``, or

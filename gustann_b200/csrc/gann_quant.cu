@@ -1,7 +1,7 @@
 // 8-bit rows with one scale each, and products of such rows.
 //
-//   quantize_rows   s_i = fl32(max_j |x_ij| / 127),  c_ij = x_ij / s_i rounded to
-//                   the nearest integer (ties to even)
+//   quantize_rows   s_i = max_j |x_ij| * (1/127) in float32,  c_ij = x_ij / s_i
+//                   rounded to the nearest integer (ties to even)
 //   matmul_i8       y_ij = (sum_k a_ik b_jk) sa_i sb_j + bias_j
 #include <algorithm>
 #include <cstdint>
@@ -46,7 +46,7 @@ struct RowScale {
 
 __device__ __forceinline__ RowScale row_scale(float amax) {
   RowScale r;
-  r.scale = isfinite(amax) ? __fdiv_rn(amax, 127.f) : __int_as_float(0x7fc00000);
+  r.scale = isfinite(amax) ? __fmul_rn(amax, 1.f / 127.f) : __int_as_float(0x7fc00000);
   r.up = r.scale < 0x1p-60f ? 0x1p64f : 1.f;
   r.s = r.scale * r.up;
   r.inv = r.s > 0.f ? __frcp_rn(r.s) : 0.f;   // 0 and NaN scales: every code 0

@@ -363,7 +363,7 @@ int gann_sort_unique_rows(const int32_t* d_ids, const float* d_dists, int64_t ro
 typedef enum { GANN_F32 = 1, GANN_F16 = 2, GANN_BF16 = 3 } gann_float;
 
 /* Rows of floats as signed 8-bit codes with one scale each, for gann_matmul_i8:
- *   scale_i = max_j |x_ij| / 127, rounded to float32
+ *   scale_i = max_j |x_ij| * c, rounded to float32; c is 1/127 rounded to float32
  *   code_ij = x_ij / scale_i rounded to the nearest integer (ties to even;
  *             the quotient is not rounded before)
  * so x_ij is about code_ij * scale_i, off by at most half a scale. A row of

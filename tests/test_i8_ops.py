@@ -19,7 +19,7 @@ def ref_quantize(x):
     x = x.float().cpu().numpy()
     amax = np.abs(x).max(1)
     with np.errstate(all="ignore"):
-        scale = np.where(np.isfinite(amax), amax / np.float32(127), np.float32(np.nan)).astype(np.float32)
+        scale = np.where(np.isfinite(amax), amax * (np.float32(1) / np.float32(127)), np.float32(np.nan)).astype(np.float32)
         q = np.rint(x.astype(np.float64) / scale.astype(np.float64)[:, None])
     live = (scale > 0)[:, None]
     return np.where(live, np.clip(q, -127, 127), 0).astype(np.int8), scale
