@@ -611,7 +611,7 @@ def beam_select(scores, logits, k: int, log_softmax: bool = False, finished=None
         if finished is not None:
             finished = finished.contiguous()
         need = C.c_int64()
-        _check(lib.gann_beam_select_workspace(g, w, v, k, dev.index or 0, C.byref(need)))
+        _check(lib.gann_beam_select_workspace(g, w, v, k, dt, C.byref(need)))
         ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
         out_s = torch.empty((g, k), dtype=torch.float32, device=dev)
         out_p = torch.empty((g, k), dtype=torch.int32, device=dev)
