@@ -111,7 +111,7 @@ def _load() -> C.CDLL:
     lib.gann_sort_unique_rows.argtypes = [vp, vp, i64, i32, vp, vp, i32, vp]
     lib.gann_quantize_rows.argtypes = [vp, i64, i64, i32, i32, vp, i64, vp, i32, vp]
     lib.gann_matmul_i8.argtypes = [vp, i64, i64, vp, vp, i64, i64, vp, vp, i32, vp, i64, i32, i32, vp]
-    lib.gann_beam_select_workspace.argtypes = [i64, i32, i32, i32, i32, C.POINTER(i64)]
+    lib.gann_beam_select_workspace.argtypes = [i64, i32, i32, i32, i32, i32, C.POINTER(i64)]
     lib.gann_beam_select.argtypes = [vp, i32, i64, i64, vp, vp, i64, i32, i32, i32, i32, i32, vp, vp, vp, vp, i64,
                                      i32, vp]
     lib.gann_reorder_states.argtypes = [C.POINTER(_State), i32, vp, i64, i32, i32, i32, vp]
@@ -611,7 +611,7 @@ def beam_select(scores, logits, k: int, log_softmax: bool = False, finished=None
         if finished is not None:
             finished = finished.contiguous()
         need = C.c_int64()
-        _check(lib.gann_beam_select_workspace(g, w, v, k, dt, C.byref(need)))
+        _check(lib.gann_beam_select_workspace(g, w, v, k, dt, int(bool(log_softmax)), C.byref(need)))
         ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
         out_s = torch.empty((g, k), dtype=torch.float32, device=dev)
         out_p = torch.empty((g, k), dtype=torch.int32, device=dev)

@@ -1164,13 +1164,13 @@ int gann_matmul_i8(const int8_t* d_a, int64_t m, int64_t a_stride, const float* 
 }
 
 int gann_beam_select_workspace(int64_t groups, int32_t beams, int32_t vocab, int32_t keep, int32_t dtype,
-                               int64_t* bytes) {
+                               int32_t log_softmax, int64_t* bytes) {
   if (!float_size(dtype))
     return set_error(GANN_EINVAL, "gann_beam_select_workspace: dtype must be GANN_F32, GANN_F16 or GANN_BF16");
   if (!bytes) return set_error(GANN_EINVAL, "gann_beam_select_workspace: null output");
   if (!select_sizes_ok(groups, beams, vocab, keep))
     return set_error(GANN_EINVAL, std::string("gann_beam_select_workspace: ") + kSelectSizes);
-  *bytes = static_cast<int64_t>(gann::beam_select_workspace(groups, beams, vocab, keep, dtype));
+  *bytes = static_cast<int64_t>(gann::beam_select_workspace(groups, beams, vocab, keep, dtype, log_softmax != 0));
   return GANN_OK;
 }
 
@@ -1208,7 +1208,7 @@ int gann_beam_select(const void* d_logits, int32_t dtype, int64_t group_stride, 
   a.out_parents = d_out_parents;
   a.out_tokens = d_out_tokens;
   a.workspace = d_workspace;
-  const size_t need = gann::beam_select_workspace(groups, beams, vocab, keep, dtype);
+  const size_t need = gann::beam_select_workspace(groups, beams, vocab, keep, dtype, log_softmax != 0);
   if (need > 0 && (!d_workspace || !aligned_to(d_workspace, 16) || workspace_bytes < static_cast<int64_t>(need)))
     return set_error(GANN_EINVAL, "gann_beam_select: the workspace must be 16-byte aligned and as large as "
                                   "gann_beam_select_workspace says");

@@ -180,7 +180,7 @@ struct SelectArgs {
   int32_t* out_tokens = nullptr;
   void* workspace = nullptr;
 };
-size_t beam_select_workspace(int64_t groups, int beams, int vocab, int keep, int dtype);
+size_t beam_select_workspace(int64_t groups, int beams, int vocab, int keep, int dtype, bool softmax);
 cudaError_t launch_beam_select(const SelectArgs& a, int sm_count, cudaStream_t st);
 cudaError_t launch_reorder_states(const gann_state* states, int count, const int32_t* parents, int64_t groups,
                                   int beams, int keep, int sm_count, cudaStream_t st);

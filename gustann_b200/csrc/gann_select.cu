@@ -122,6 +122,12 @@ struct Key2 {
   }
 };
 
+// Whether a lane keeps the larger key at a step of a bitonic sort (largest
+// first) over lanes: bit log2(size) of the lane equals bit log2(stride).
+__device__ __forceinline__ bool keeps_larger(int lane, int size, int stride) {
+  return size >= 32 ? (lane & stride) == 0 : ((lane ^ (lane / (size / stride))) & stride) == 0;
+}
+
 // Bitonic sort of 32 N keys by one warp, largest first; key n * 32 + lane is
 // k[n] of the lane.
 template <int N, typename K>
@@ -130,25 +136,19 @@ __device__ __forceinline__ void warp_sort(K (&k)[N], int lane) {
   for (int size = 2; size <= 32 * N; size <<= 1) {
 #pragma unroll
     for (int stride = size >> 1; stride > 0; stride >>= 1) {
-      if (stride >= 32) {
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
+      for (int n = 0; n < N; ++n) {
+        const bool down = size < 32 || ((n * 32) & size) == 0;
+        if (stride >= 32) {
           const int o = n ^ (stride / 32);
-          if (o > n) {
-            const bool down = ((n * 32) & size) == 0;
-            if (k[o].above(k[n]) == down) {
-              const K t = k[n];
-              k[n] = k[o];
-              k[o] = t;
-            }
+          if (o > n && k[o].above(k[n]) == down) {
+            const K t = k[n];
+            k[n] = k[o];
+            k[o] = t;
           }
-        }
-      } else {
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
+        } else {
           const K o = k[n].from(stride);
-          const bool down = ((n * 32 + lane) & size) == 0, low = (lane & stride) == 0;
-          if (o.above(k[n]) == (down == low)) k[n] = o;
+          if (o.above(k[n]) == (keeps_larger(lane, size, stride) == down)) k[n] = o;
         }
       }
     }
@@ -165,6 +165,25 @@ __device__ __forceinline__ uint32_t warp_rth(uint32_t u, int r, int lane) {
   }
   return w;
 }
+
+// The warp's 32 values sorted, largest first.
+__device__ __forceinline__ float warp_sort32(float v, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      const float o = __shfl_xor_sync(kFull, v, stride);
+      v = keeps_larger(lane, size, stride) ? fmaxf(v, o) : fminf(v, o);
+    }
+  return v;
+}
+
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2e = 1.4426950408889634f;
 
 // Sum of one int a thread over the block; `red` holds a word for each warp.
 // The barriers around it make it safe to call in a loop.
@@ -183,213 +202,406 @@ __device__ __forceinline__ int block_sum(int c, int* red) {
 
 __device__ __forceinline__ bool live(float score) { return fabsf(score) < INFINITY; }
 
-// ------------------------------------------------------------ split rows
-// Large vocabularies: a block takes a segment of one row, keeps it in
-// registers, sums its exponentials against the segment's maximum and writes
-// the segment's best candidates; merge_kernel joins the segments.
-//
-// Threshold: every warp finds the r-th largest of its 32 lanes' maxima, r =
-// ceil(keep / 8); the least of the 8 warps' values has at least `keep`
-// elements at or above it, so nothing below it can be kept. On data in no
-// particular order a few dozen of 8192 elements pass it. More than kHits
-// (equal values, sorted rows in the tail) are cut to exactly `keep` by
-// bisection over the value and then the index.
-constexpr int kSplitWarps = 8;
-constexpr int kSplitThreads = kSplitWarps * kWarp;
+// Sorts the warp's keys get(0 .. total - 1) and stores the best `keep`.
+template <int P, typename K, typename Get>
+__device__ __forceinline__ void sort_keys(K* kept, int total, int keep, int lane, Get&& get) {
+  K k[P];
+#pragma unroll
+  for (int n = 0; n < P; ++n) k[n] = n * kWarp + lane < total ? get(n * kWarp + lane) : K{};
+  warp_sort<P>(k, lane);
+  __syncwarp();
+#pragma unroll
+  for (int n = 0; n < P; ++n)
+    if (n * kWarp + lane < min(total, keep)) kept[n * kWarp + lane] = k[n];
+  __syncwarp();
+}
+// LONG: up to 256 keys, else up to 64.
+template <bool LONG, typename K, typename Get>
+__device__ __forceinline__ void sort_some(K* kept, int total, int keep, int lane, Get&& get) {
+  __syncwarp();
+  if (total <= 32) sort_keys<1>(kept, total, keep, lane, get);
+  else if (!LONG || total <= 64) sort_keys<2>(kept, total, keep, lane, get);
+  else if (total <= 128) sort_keys<4>(kept, total, keep, lane, get);
+  else sort_keys<8>(kept, total, keep, lane, get);
+}
+// Candidates that a warp holds at a time, kept ones among them, in the two
+// forms of the kernels below: keep <= 16, and more.
+constexpr int kShortKeep = 16;
+template <bool LONG>
+struct Held {
+  static constexpr int value = LONG ? kHits : 64;
+};
+
+// --------------------------------------------------------- segments of rows
+// Large vocabularies, and every call with log-softmax: a warp streams a
+// segment of one row, four 16-byte vectors a lane at a time with the next four
+// on their way, and keeps, without any barrier,
+//   - for each lane the running maximum and the sum of exp(x - maximum) (terms
+//     in float32, at most 32 at a time, joined in 64 bits);
+//   - the list of the best candidates. The first tile sets its threshold: of
+//     the 32 lanes' maxima the keep-th largest (keep <= 16), or among the 128
+//     vectors' maxima by bisection, has `keep` elements at or above it. Lanes
+//     mark their elements at or above the threshold; the marked ones are
+//     compared with the least kept key and listed, one a lane at a time. The
+//     list is sorted and cut when it is full, which raises the threshold.
+// A segment writes its `keep` best and its sum; merge_kernel joins them.
+constexpr int kRowWarps = 4, kRowVecs = 4;
+constexpr int kRowTile = kRowVecs * kWarp;   // vectors
 
 struct SegStat {
   double max, sum;
 };
 
-template <typename T, int E>
-__device__ __forceinline__ void load_segment(uint4 (&raw)[E / Raw<T>::n], const T* row, int vocab, int head, int64_t base) {
+template <typename T, bool SOFTMAX, bool LONG>
+__global__ void __launch_bounds__(kRowWarps* kWarp, 5) row_kernel(const T* __restrict__ logits, int64_t gstride,
+                                                               int64_t bstride, const float* __restrict__ scores,
+                                                               const uint8_t* __restrict__ finished, int64_t rows,
+                                                               int beams, int vocab, int keep, int segs, int seg_tiles,
+                                                               Key1* __restrict__ out, SegStat* __restrict__ stats) {
   constexpr int N = Raw<T>::n;
   constexpr uint32_t ninf = Raw<T>::neg_inf;
-#pragma unroll
-  for (int i = 0; i < E / N; ++i) {
-    const int64_t p = base + (static_cast<int64_t>(i) * kSplitThreads + threadIdx.x) * N - head;   // first element
-    raw[i] = make_uint4(ninf, ninf, ninf, ninf);
-    if (p >= 0 && p + N <= vocab) {
-      raw[i] = __ldcs(reinterpret_cast<const uint4*>(row + p));
-    } else if (p + N > 0 && p < vocab) {
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (p + j >= 0 && p + j < vocab) Raw<T>::put(raw[i], j, row + p + j);
-    }
-  }
-}
+  constexpr int kCap = Held<LONG>::value;
+  __shared__ Key1 lists[kRowWarps][kCap];
+  const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * kRowWarps + warp;
+  if (item >= rows * segs) return;
+  const int64_t rw = item / segs;
+  const int seg = static_cast<int>(item - rw * segs);
+  if (!live(scores[rw]) || (finished && finished[rw])) return;
+  const int64_t g = rw / beams;
+  const T* row = logits + g * gstride + (rw - g * beams) * bstride;
+  const int head = static_cast<int>((reinterpret_cast<uintptr_t>(row) % 16) / sizeof(T));
+  // elements of the row before its first whole vector make a partial one; the
+  // segment's first element, counted from that vector's start
+  const int64_t first = static_cast<int64_t>(seg) * seg_tiles * kRowTile * N - head;
 
-template <typename T, int E, bool SOFTMAX>
-__global__ void __launch_bounds__(kSplitThreads, 4) split_kernel(const T* __restrict__ logits, int64_t gstride,
-                                                                 int64_t bstride, const float* __restrict__ scores,
-                                                                 const uint8_t* __restrict__ finished, int64_t rows,
-                                                                 int beams, int vocab, int keep, int segs,
-                                                                 Key1* __restrict__ out, SegStat* __restrict__ stats) {
-  constexpr int N = Raw<T>::n, V = E / N;
-  __shared__ uint64_t hits[kHits];
-  __shared__ uint32_t rth[kSplitWarps], top[kSplitWarps];
-  __shared__ double part[kSplitWarps];
-  __shared__ int red[kSplitWarps], count;
-  const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
-  const int r = (keep + kSplitWarps - 1) / kSplitWarps;
-  const int64_t total = rows * segs;
-  for (int64_t item = blockIdx.x; item < total; item += gridDim.x) {
-    const int64_t rw = item / segs;
-    const int64_t g = rw / beams;
-    const int b = static_cast<int>(rw - g * beams);
-    if (!live(scores[rw]) || (finished && finished[rw])) continue;
-    const T* row = logits + g * gstride + b * bstride;
-    const int head = static_cast<int>((reinterpret_cast<uintptr_t>(row) % 16) / sizeof(T));
-    const int64_t base = (item - rw * segs) * (static_cast<int64_t>(kSplitThreads) * E);
-    uint4 raw[V];
-    load_segment<T, E>(raw, row, vocab, head, base);
-    float vm[V], mx = -INFINITY;
+  auto load = [&](uint4 (&raw)[kRowVecs], int tile) {
+    const int64_t p0 = first + static_cast<int64_t>(tile) * kRowTile * N;
+    if (p0 >= 0 && p0 + kRowTile * N <= vocab) {
+      const uint4* v = reinterpret_cast<const uint4*>(row + p0) + lane;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      vm[i] = Raw<T>::max(raw[i]);
+      for (int i = 0; i < kRowVecs; ++i) raw[i] = __ldcs(v + i * kWarp);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kRowVecs; ++i) {
+        const int64_t p = p0 + (i * kWarp + lane) * N;
+        raw[i] = make_uint4(ninf, ninf, ninf, ninf);
+        if (p >= 0 && p + N <= vocab) {
+          raw[i] = __ldcs(reinterpret_cast<const uint4*>(row + p));
+        } else if (p + N > 0 && p < vocab) {
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+            if (p + j >= 0 && p + j < vocab) Raw<T>::put(raw[i], j, row + p + j);
+        }
+      }
+    }
+  };
+
+  Key1* list = lists[warp];
+  Key1 floor{0};   // the least kept key once `keep` are known
+  int cnt = 0;
+  float thr = -INFINITY, m = -INFINITY;
+  auto cut = [&]() {
+    sort_some<LONG>(list, cnt, keep, lane, [&](int i) { return list[i]; });
+    cnt = min(cnt, keep);
+    if (cnt < keep) return;
+    floor = list[keep - 1];
+    thr = unord32(static_cast<uint32_t>(floor.a >> 32));
+  };
+  double sum = 0.0;
+  const int64_t last = (vocab - first + static_cast<int64_t>(kRowTile) * N - 1) / (static_cast<int64_t>(kRowTile) * N);
+  const int tiles = static_cast<int>(min(static_cast<int64_t>(seg_tiles), last));   // <= 0: nothing here
+  uint4 cur[kRowVecs], nxt[kRowVecs];
+  if (tiles > 0) load(cur, 0);
+  for (int t = 0; t < tiles; ++t) {
+    if (t + 1 < tiles) load(nxt, t + 1);
+    float vm[kRowVecs], mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kRowVecs; ++i) {
+      vm[i] = Raw<T>::max(cur[i]);
       mx = fmaxf(mx, vm[i]);
     }
-    if (mx == INFINITY) {   // infinite entries are masked: the maximum without them
+    if (mx == INFINITY) {   // infinite entries are masked: the maxima without them
       mx = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
+      for (int i = 0; i < kRowVecs; ++i) {
         vm[i] = -INFINITY;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          const float x = Raw<T>::at(raw[i], j);
+          const float x = Raw<T>::at(cur[i], j);
           if (x < INFINITY) vm[i] = fmaxf(vm[i], x);
         }
         mx = fmaxf(mx, vm[i]);
       }
     }
-    const uint32_t u = ord32(mx);
-    const uint32_t wm = __reduce_max_sync(kFull, u), wr = warp_rth(u, r, lane);
-    if (lane == 0) {
-      rth[warp] = wr;
-      top[warp] = wm;
-    }
-    if (tid == 0) count = 0;
-    __syncthreads();
-    uint32_t lo = rth[0], hi = top[0];
+    if (t == 0) {
+      if (!LONG) {
+        thr = __shfl_sync(kFull, warp_sort32(mx, lane), keep - 1);
+      } else {
+        uint32_t lo = 0x007fffffu, hi = __reduce_max_sync(kFull, ord32(mx)) + 1;   // lo: ord32(-inf)
+        for (int r = 0; r < 32 && hi - lo > 1; ++r) {
+          const uint32_t mid = lo + (hi - lo) / 2;
+          const float x = unord32(mid);
+          int n = 0;
 #pragma unroll
-    for (int w = 1; w < kSplitWarps; ++w) {
-      lo = min(lo, rth[w]);
-      hi = max(hi, top[w]);
-    }
-    const float m = unord32(hi);
-    auto index_of = [&](int i, int j) {
-      return static_cast<uint32_t>(base + (static_cast<int64_t>(i) * kSplitThreads + tid) * N + j - head);
-    };
-    auto collect = [&](float thr, uint32_t floor_key, uint32_t last_index) {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (vm[i] >= thr) {
-#pragma unroll
-          for (int j = 0; j < N; ++j) {
-            const float x = Raw<T>::at(raw[i], j);
-            if (x >= thr && fabsf(x) < INFINITY) {
-              const uint32_t k = ord32(x), id = index_of(i, j);
-              if (k > floor_key || id <= last_index) {
-                const int at = atomicAdd(&count, 1);
-                if (at < kHits) hits[at] = (static_cast<uint64_t>(k) << 32) | ~id;
-              }
-            }
-          }
+          for (int i = 0; i < kRowVecs; ++i) n += __popc(__ballot_sync(kFull, vm[i] >= x));
+          if (n >= keep) lo = mid;
+          else hi = mid;
+          if (n == keep) break;
         }
-    };
-    collect(unord32(lo), 0, 0);
+        thr = unord32(lo);
+      }
+    }
+    const int64_t p0 = first + static_cast<int64_t>(t) * kRowTile * N;
+    if (__any_sync(kFull, mx >= thr)) {
+      uint32_t mark = 0;
+#pragma unroll
+      for (int i = 0; i < kRowVecs; ++i)
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (Raw<T>::at(cur[i], j) >= thr) mark |= 1u << (i * N + j);
+      while (__any_sync(kFull, mark)) {
+        if (cnt > kCap - kWarp) cut();
+        const int e = __ffs(mark) - 1;
+        const int64_t p = p0 + ((e / N) * kWarp + lane) * N + e % N;
+        const float x = mark && p >= 0 && p < vocab ? Raw<T>::one(row + p) : kNan;
+        const Key1 k{(static_cast<uint64_t>(ord32(x)) << 32) | ~static_cast<uint32_t>(p)};
+        const bool take = fabsf(x) < INFINITY && k.above(floor);
+        const unsigned pass = __ballot_sync(kFull, take);
+        if (take) list[cnt + __popc(pass & ((1u << lane) - 1u))] = k;
+        cnt += __popc(pass);
+        mark &= mark - 1;
+      }
+    }
     if (SOFTMAX) {
-      // sum of exp(x - m), at most 32 terms a thread; the maximum's term is 1
-      float sum = 0.f;
+      if (mx > m) {
+        sum *= static_cast<double>(fast_exp2((m - mx) * kLog2e));
+        m = mx;
+      }
+      float part = 0.f;
       if (m > -INFINITY) {
-        constexpr float kLog2e = 1.4426950408889634f;
 #pragma unroll
-        for (int i = 0; i < V; ++i)
+        for (int i = 0; i < kRowVecs; ++i)
 #pragma unroll
-          for (int j = 0; j < N; ++j) sum += exp2f((Raw<T>::at(raw[i], j) - m) * kLog2e);
-        if (!(sum < INFINITY)) {   // a NaN or an infinite entry: again without them
-          sum = 0.f;
+          for (int j = 0; j < N; ++j) part += fast_exp2((Raw<T>::at(cur[i], j) - m) * kLog2e);
+        if (!(part < INFINITY)) {   // a NaN or an infinite entry: again without them
+          part = 0.f;
 #pragma unroll
-          for (int i = 0; i < V; ++i)
+          for (int i = 0; i < kRowVecs; ++i)
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-              const float x = Raw<T>::at(raw[i], j);
-              if (fabsf(x) < INFINITY) sum += exp2f((x - m) * kLog2e);
+              const float x = Raw<T>::at(cur[i], j);
+              if (fabsf(x) < INFINITY) part += fast_exp2((x - m) * kLog2e);
             }
         }
       }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-      if (lane == 0) part[warp] = sum;
+      sum += static_cast<double>(part);
     }
-    __syncthreads();
-    int c = count;
-    if (c > kHits) {
-      // exactly `keep`: the key of the keep-th largest value, then the index
-      // up to which its equals are taken
-      auto at_least = [&](uint32_t k) {
-        int n = 0;
 #pragma unroll
-        for (int i = 0; i < V; ++i)
+    for (int i = 0; i < kRowVecs; ++i) cur[i] = nxt[i];
+  }
+  if (cnt > keep) cut();
+  __syncwarp();
+  for (int j = lane; j < keep; j += kWarp) out[item * keep + j] = j < cnt ? list[j] : Key1{0};
+  if (SOFTMAX) {
+    const float mm = unord32(__reduce_max_sync(kFull, ord32(m)));
+    sum = m > -INFINITY ? sum * static_cast<double>(fast_exp2((m - mm) * kLog2e)) : 0.0;
 #pragma unroll
-          for (int j = 0; j < N; ++j) {
-            const float x = Raw<T>::at(raw[i], j);
-            n += fabsf(x) < INFINITY && ord32(x) >= k;
-          }
-        return block_sum<kSplitWarps>(n, red);
-      };
-      uint32_t top_key = hi + 1;   // fewer than keep at or above
-      while (top_key - lo > 1) {
-        const uint32_t mid = lo + (top_key - lo) / 2;
-        if (at_least(mid) >= keep) lo = mid;
-        else top_key = mid;
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+    if (lane == 0) stats[item] = {static_cast<double>(mm), sum};
+  }
+}
+
+// ------------------------------------------------------------ whole groups
+// Many groups, no softmax: a warp takes a whole group, in tiles of 32 (16)
+// elements a lane in registers, vectors of 16 bytes (single elements when rows
+// are not whole vectors). f = fl32(x + S_b) orders candidates as their 64-bit
+// values do, up to equality. The first tile sets a threshold of f: the keep-th
+// largest of the lanes' maxima (keep <= 16), or one bisected until between
+// `keep` and 128 elements pass. Lanes mark the elements with x >= thr - S_b (a
+// little less, so none with f >= thr is missed); the marked ones are valued
+// in 64 bits, compared with the least kept key and listed.
+constexpr int kGroupWarps = 4;
+
+template <typename T, int VW>
+struct Vec {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* p) { v = __ldcs(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ float at(int j) const { return Raw<T>::at(v, j); }
+  __device__ __forceinline__ float max() const { return Raw<T>::max(v); }
+};
+template <typename T>
+struct Vec<T, 1> {
+  float v;
+  __device__ __forceinline__ void load(const T* p) { v = Raw<T>::one(p); }
+  __device__ __forceinline__ float at(int) const { return v; }
+  __device__ __forceinline__ float max() const { return v; }
+};
+
+template <typename T, int VW, bool LONG>
+__global__ void __launch_bounds__(kGroupWarps* kWarp, LONG ? 4 : 6) group_kernel(
+    const T* __restrict__ logits, int64_t gstride, int64_t bstride, const float* __restrict__ scores,
+    const uint8_t* __restrict__ finished, int64_t groups, int beams, int vocab, int keep, int end_token, uint32_t magic,
+    int shift, float* __restrict__ out_s, int32_t* __restrict__ out_p, int32_t* __restrict__ out_t) {
+  constexpr int NV = VW == 1 ? 16 : 32 / VW, kCap = Held<LONG>::value;
+  __shared__ Key2 lists[kGroupWarps][kCap];
+  __shared__ float cs[kGroupWarps][kBeamMax];
+  const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
+  const int64_t g = static_cast<int64_t>(blockIdx.x) * kGroupWarps + warp;
+  if (g >= groups) return;
+  const T* base = logits + g * gstride;
+  const float* sc = scores + g * beams;
+  float* c = cs[warp];
+  Key2* list = lists[warp];
+  const uint32_t vr = static_cast<uint32_t>(vocab) / VW, nvec = vr * beams;
+  const bool joined = bstride == vocab;
+  // row of a vector: division by the row's length as a product (magic =
+  // ceil(2^(32+shift) / vr), exact below 2^31)
+  auto row_of = [&](uint32_t v) { return (magic ? __umulhi(v, magic) : v) >> shift; };
+  Vec<T, VW> raw[NV];
+  auto load = [&](uint32_t t0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t v = t0 + i * kWarp + lane;
+      if (v < nvec) {
+        if (joined) {
+          raw[i].load(base + static_cast<int64_t>(v) * VW);
+        } else {
+          const uint32_t b = row_of(v);
+          raw[i].load(base + b * bstride + static_cast<int64_t>(v - b * vr) * VW);
+        }
       }
-      const int want = keep - at_least(lo + 1);
-      int64_t i0 = base - N, i1 = base + static_cast<int64_t>(kSplitThreads) * E;   // want in (i0, i1]
-      while (i1 - i0 > 1) {
-        const int64_t mid = i0 + (i1 - i0) / 2;
-        int n = 0;
+    }
+  };
+  load(0);
+  for (int b = lane; b < beams; b += kWarp) {
+    const float s = sc[b];
+    c[b] = live(s) && !(finished && finished[g * beams + b]) ? s : kNan;
+  }
+  __syncwarp();
+  int cnt = 0;
+  Key2 floor{0, 0};   // the least kept key once `keep` are known
+  float thr = -INFINITY;
+  auto cut = [&]() {
+    sort_some<LONG>(list, cnt, keep, lane, [&](int i) { return list[i]; });
+    cnt = min(cnt, keep);
+    if (cnt < keep) return;
+    floor = list[keep - 1];
+    thr = static_cast<float>(unord64(floor.a));
+  };
+  for (uint32_t t0 = 0; t0 < nvec; t0 += NV * kWarp) {
+    if (t0) load(t0);
+    float cb[NV];   // NaN: a row without elements, or nothing there
 #pragma unroll
-        for (int i = 0; i < V; ++i)
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t v = t0 + i * kWarp + lane;
+      cb[i] = v < nvec ? c[row_of(v)] : kNan;
+    }
+    if (t0 == 0) {
+      if (!LONG) {
+        // rounding keeps order, so one sum a vector; masked entries that are
+        // +infinity have to be left out
+        float mx = -INFINITY;
 #pragma unroll
-          for (int j = 0; j < N; ++j) {
-            const float x = Raw<T>::at(raw[i], j);
-            const int64_t p = base + (static_cast<int64_t>(i) * kSplitThreads + tid) * N + j - head;
-            n += fabsf(x) < INFINITY && ord32(x) == lo && p <= mid;
+        for (int i = 0; i < NV; ++i) mx = fmaxf(mx, __fadd_rn(raw[i].max(), cb[i]));
+        if (mx == INFINITY) {
+          mx = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < VW; ++j)
+              if (raw[i].at(j) < INFINITY) mx = fmaxf(mx, __fadd_rn(raw[i].at(j), cb[i]));
+        }
+        thr = __shfl_sync(kFull, warp_sort32(mx, lane), keep - 1);
+      } else {
+        // bisection by value, then (far from done) over the order of floats
+        float hi = -INFINITY, lo = -INFINITY, low = INFINITY;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int j = 0; j < VW; ++j) {
+            const float x = raw[i].at(j), f = __fadd_rn(x, cb[i]);
+            if (fabsf(x) < INFINITY && fabsf(f) < INFINITY) {
+              hi = fmaxf(hi, f);
+              low = fminf(low, f);
+            }
           }
-        if (block_sum<kSplitWarps>(n, red) >= want) i1 = mid;
-        else i0 = mid;
+        hi = unord32(__reduce_max_sync(kFull, ord32(hi)));
+        float mid = -unord32(__reduce_max_sync(kFull, ord32(-low)));
+        for (int r = 0; r < 24 && hi > mid; ++r) {
+          int n = 0;
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+            if (i * kWarp < nvec) {
+#pragma unroll
+              for (int j = 0; j < VW; ++j) n += __fadd_rn(raw[i].at(j), cb[i]) >= mid && raw[i].at(j) < INFINITY;
+            }
+          n = __reduce_add_sync(kFull, n);
+          if (n >= keep) {
+            lo = mid;
+            if (n <= 128) break;
+          } else {
+            hi = mid;
+          }
+          const uint32_t a = ord32(lo), b = ord32(hi);
+          if (b - a <= 1) break;
+          mid = r < 10 && lo > -INFINITY ? 0.5f * lo + 0.5f * hi : unord32(a + (b - a) / 2);
+          if (!(mid > lo && mid < hi)) mid = unord32(a + (b - a) / 2);
+        }
+        thr = lo;
       }
-      if (tid == 0) count = 0;
-      __syncthreads();
-      collect(unord32(lo), lo, static_cast<uint32_t>(i1));
-      __syncthreads();
-      c = count;
     }
-    Key1* o = out + item * keep;
-    if (warp == 0) {
-      auto sorted = [&](auto tag) {
-        constexpr int P = decltype(tag)::value;
-        Key1 k[P];
+    uint32_t mark = 0;
+    const float below = thr - fabsf(thr) * 0x1p-23f;   // by half a step of thr at least
 #pragma unroll
-        for (int n = 0; n < P; ++n) k[n] = {n * kWarp + lane < c ? hits[n * kWarp + lane] : 0};
-        warp_sort<P>(k, lane);
+    for (int i = 0; i < NV; ++i) {
+      const float least = __fadd_rd(below, -cb[i]);
 #pragma unroll
-        for (int n = 0; n < P; ++n)
-          if (n * kWarp + lane < keep) o[n * kWarp + lane] = k[n];
-        for (int n = P * kWarp + lane; n < keep; n += kWarp) o[n] = {0};
-      };
-      if (c <= 32) sorted(std::integral_constant<int, 1>{});
-      else if (c <= 64) sorted(std::integral_constant<int, 2>{});
-      else if (c <= 128) sorted(std::integral_constant<int, 4>{});
-      else sorted(std::integral_constant<int, 8>{});
-    } else if (SOFTMAX && warp == 1 && lane == 0) {
-      double s = 0.0;
-#pragma unroll
-      for (int w = 0; w < kSplitWarps; ++w) s += part[w];
-      stats[item] = {m, s};
+      for (int j = 0; j < VW; ++j)
+        if (raw[i].at(j) >= least) mark |= 1u << (i * VW + j);
     }
-    __syncthreads();
+    int b0 = 0;
+    while (true) {
+      bool take = mark != 0;
+      double v = 0.0;
+      uint32_t id = 0;
+      if (__any_sync(kFull, take)) {
+        if (take) {
+          const int e = __ffs(mark) - 1;
+          id = (t0 + (e / VW) * kWarp + lane) * VW + e % VW;
+          const uint32_t b = row_of(id / VW);
+          const float x = Raw<T>::one(base + b * bstride + (id - b * vocab));
+          take = fabsf(x) < INFINITY;
+          v = static_cast<double>(c[b]) + static_cast<double>(x);
+          mark &= mark - 1;
+        }
+      } else {
+        if (!finished || t0 || b0 >= beams) break;
+        const int b = b0 + lane;
+        take = b < beams && isnan(c[b]) && live(sc[b]);
+        if (take) {
+          v = static_cast<double>(sc[b]);
+          id = static_cast<uint32_t>(b) * vocab + end_token;
+        }
+        b0 += kWarp;
+      }
+      if (cnt > kCap - kWarp) cut();
+      const Key2 k{ord64(v), ~id};
+      take = take && k.above(floor);
+      const unsigned pass = __ballot_sync(kFull, take);
+      if (take) list[cnt + __popc(pass & ((1u << lane) - 1u))] = k;
+      cnt += __popc(pass);
+    }
+  }
+  if (cnt) cut();
+  const int nkept = cnt;
+  for (int j = lane; j < keep; j += kWarp) {
+    const bool ok = j < nkept;
+    const Key2 k = ok ? list[j] : Key2{0, 0};
+    const uint32_t idx = ~k.b, b = ok ? idx / static_cast<uint32_t>(vocab) : 0u;
+    out_s[g * keep + j] = ok ? static_cast<float>(unord64(k.a)) : -INFINITY;
+    out_p[g * keep + j] = ok ? static_cast<int32_t>(b) : -1;
+    out_t[g * keep + j] = ok ? static_cast<int32_t>(idx - b * vocab) : -1;
   }
 }
 
@@ -668,93 +880,6 @@ __device__ __forceinline__ void set_cmax(SelShared& sh, int beams) {
   }
 }
 
-// Groups of at most 32 NW E elements: one block each, the group in registers.
-template <typename T, int NW, int E>
-__global__ void __launch_bounds__(NW* kWarp) group_kernel(const T* __restrict__ logits, int64_t gstride,
-                                                          int64_t bstride, const float* __restrict__ scores,
-                                                          const uint8_t* __restrict__ finished, int64_t groups,
-                                                          int beams, int vocab, int keep, int softmax, int end_token,
-                                                          int vec, uint32_t magic, float* __restrict__ out_s,
-                                                          int32_t* __restrict__ out_p, int32_t* __restrict__ out_t) {
-  constexpr int NT = NW * kWarp, N = Raw<T>::n;
-  __shared__ SelShared sh;
-  const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
-  const int total = beams * vocab;
-  for (int64_t g = blockIdx.x; g < groups; g += gridDim.x) {
-    const T* base = logits + g * gstride;
-    const float* sc = scores + g * beams;
-    if (softmax) {
-      for (int b = warp; b < beams; b += NW) {
-        const T* row = base + b * bstride;
-        float mx = -INFINITY;
-        for (int t = lane; t < vocab; t += kWarp) {
-          const float x = Raw<T>::one(row + t);
-          if (x < INFINITY) mx = fmaxf(mx, x);
-        }
-        mx = unord32(__reduce_max_sync(kFull, ord32(mx)));
-        double sum = 0.0;
-        for (int t = lane; t < vocab; t += kWarp) {
-          const float x = Raw<T>::one(row + t);
-          if (fabsf(x) < INFINITY) sum += exp2f((x - mx) * 1.4426950408889634f);
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-        if (lane == 0) set_row(sh, b, sc[b], finished && finished[g * beams + b], true, mx, sum);
-      }
-    } else {
-      for (int b = tid; b < beams; b += NT) set_row(sh, b, sc[b], finished && finished[g * beams + b], false, 0.f, 0.0);
-    }
-    __syncthreads();
-    set_cmax(sh, beams);
-    // f[i]: with vec, elements are 16-byte vectors of the group's rows
-    float f[E];
-    auto name = [&](int i) {
-      return vec ? static_cast<uint32_t>((i / N * NT + tid) * N + i % N) : static_cast<uint32_t>(i * NT + tid);
-    };
-    // row of an element or vector: division by the row's length as a product
-    // (exact: e < 2^14, length <= 2^13)
-    auto row_of = [&](uint32_t e) { return magic ? __umulhi(e, magic) : e; };
-    if (vec) {
-      const int vr = vocab / N;
-#pragma unroll
-      for (int i = 0; i < E / N; ++i) {
-        const uint32_t v = i * NT + tid;
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        float c = kNan;
-        if (v * N < static_cast<uint32_t>(total)) {
-          const uint32_t b = row_of(v);
-          raw = __ldcs(reinterpret_cast<const uint4*>(base + b * bstride + (v - b * vr) * N));
-          c = sh.c[b];
-        }
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const float x = Raw<T>::at(raw, j);
-          f[i * N + j] = __fmaf_rn(x, 0.f, __fadd_rn(x, c));   // NaN when x is not finite
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const uint32_t e = i * NT + tid;
-        f[i] = kNan;
-        if (e < static_cast<uint32_t>(total)) {
-          const uint32_t b = row_of(e);
-          const float x = Raw<T>::one(base + b * bstride + (e - b * vocab));
-          f[i] = __fmaf_rn(x, 0.f, __fadd_rn(x, sh.c[b]));
-        }
-      }
-    }
-    auto value = [&](uint32_t e, double& v, uint32_t& idx) {
-      const uint32_t b = e / static_cast<uint32_t>(vocab);
-      v = row_value(sh, b, Raw<T>::one(base + b * bstride + (e - b * vocab)));
-      idx = e;
-    };
-    block_select<NW, E>(sh, f, beams, vocab, keep, end_token, true, name, value, sc);
-    write_kept<NW>(sh, g, vocab, keep, out_s, out_p, out_t);
-    __syncthreads();
-  }
-}
-
 // The segments' candidates of one group joined: one block a group, tiles of
 // 32 x 8 x 16 candidates.
 constexpr int kMergeWarps = 8, kMergeElems = 16;
@@ -852,29 +977,37 @@ __global__ void __launch_bounds__(256) reorder_kernel(const __grid_constant__ St
 
 namespace {
 
-// How a call is run. A group of at most 8192 elements is one block's (group
-// kernel: one launch, nothing written but the result); larger ones are split
-// into rows' segments and joined. Elements a thread of the split kernel: as
-// few as hold a row, and no fewer than 8.
+// How a call is run. Without softmax a warp can take a whole group: one
+// launch, nothing written but the result. That needs enough groups to fill the
+// GPU, or groups so small that one warp is done at once. Everything else is
+// split: rows into segments, a warp each, as many as the GPU holds at a time,
+// and joined by a second kernel.
+constexpr int kResidentWarps = 148 * 20;
+constexpr int kSmallGroup = 4096;      // bytes of a group that a lone warp reads in one tile
+
 struct SelectPlan {
   bool split = false;
-  int elems = 32, segs = 0;
+  int segs = 0, seg_tiles = 0;
 };
 
-SelectPlan plan_select(int beams, int vocab, int dtype) {
+SelectPlan plan_select(int64_t groups, int beams, int vocab, int dtype, bool softmax) {
   SelectPlan p;
-  if (static_cast<int64_t>(beams) * vocab <= 8 * kWarp * 32) return p;
-  p.split = true;
-  const int64_t span = static_cast<int64_t>(vocab) + (dtype == GANN_F32 ? 3 : 7);   // a row may start inside a vector
-  p.elems = span <= kSplitThreads * 8 ? 8 : span <= kSplitThreads * 16 ? 16 : 32;
-  p.segs = static_cast<int>((span + kSplitThreads * p.elems - 1) / (kSplitThreads * p.elems));
+  const int elem = dtype == GANN_F32 ? 4 : 2, n = 16 / elem;
+  const int64_t bytes = static_cast<int64_t>(beams) * vocab * elem;
+  p.split = softmax || !(bytes <= kSmallGroup || groups >= kResidentWarps / 4);
+  if (!p.split) return p;
+  const int64_t rows = std::max<int64_t>(1, groups * beams);
+  const int64_t tiles = (static_cast<int64_t>(vocab) + n - 1 + kRowTile * n - 1) / (kRowTile * n);   // a row may start inside a vector
+  const int64_t want = std::max<int64_t>(1, kResidentWarps / rows);
+  p.seg_tiles = static_cast<int>((tiles + want - 1) / want);
+  p.segs = static_cast<int>((tiles + p.seg_tiles - 1) / p.seg_tiles);
   return p;
 }
 
 }  // namespace
 
-size_t beam_select_workspace(int64_t groups, int beams, int vocab, int keep, int dtype) {
-  const SelectPlan p = plan_select(beams, vocab, dtype);
+size_t beam_select_workspace(int64_t groups, int beams, int vocab, int keep, int dtype, bool softmax) {
+  const SelectPlan p = plan_select(groups, beams, vocab, dtype, softmax);
   if (!p.split) return 0;
   const size_t items = static_cast<size_t>(groups) * beams * p.segs;
   return items * (sizeof(SegStat) + sizeof(Key1) * keep);
@@ -883,48 +1016,46 @@ size_t beam_select_workspace(int64_t groups, int beams, int vocab, int keep, int
 namespace {
 
 template <typename T>
-cudaError_t run_group(const SelectArgs& a, int sm_count, cudaStream_t st) {
+cudaError_t run_group(const SelectArgs& a, cudaStream_t st) {
   constexpr int n = Raw<T>::n;
-  const int total = a.beams * a.vocab;
   const bool vec = a.vocab % n == 0 && a.group_stride % n == 0 && a.beam_stride % n == 0 &&
                    reinterpret_cast<uintptr_t>(a.logits) % 16 == 0;
   const uint32_t div = static_cast<uint32_t>(vec ? a.vocab / n : a.vocab);
-  const uint32_t magic = div == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + div - 1) / div);
-  auto run = [&](auto fn, int warps) {
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.groups, static_cast<int64_t>(sm_count) * 256));
-    fn<<<grid, warps * kWarp, 0, st>>>(static_cast<const T*>(a.logits), a.group_stride, a.beam_stride, a.scores,
-                                       a.finished, a.groups, a.beams, a.vocab, a.keep, a.softmax, a.end_token, vec,
-                                       magic, a.out_scores, a.out_parents, a.out_tokens);
+  // magic and shift of a division by `div` that is exact below 2^31
+  uint32_t magic = 0;
+  int shift = 0;
+  while ((1u << shift) < div) ++shift;
+  if ((1u << shift) != div) {
+    --shift;
+    magic = static_cast<uint32_t>(((1ull << (32 + shift)) + div - 1) / div);
+  }
+  auto run = [&](auto fn) {
+    fn<<<static_cast<unsigned>((a.groups + kGroupWarps - 1) / kGroupWarps), kGroupWarps * kWarp, 0, st>>>(
+        static_cast<const T*>(a.logits), a.group_stride, a.beam_stride, a.scores, a.finished, a.groups, a.beams,
+        a.vocab, a.keep, a.end_token, magic, shift, a.out_scores, a.out_parents, a.out_tokens);
     return cudaGetLastError();
   };
-  // the threshold wants keep <= 32 a warp; the smallest block that holds the
-  // group
-  if (total <= 256 && a.keep <= 32) return run(group_kernel<T, 1, 8>, 1);
-  if (total <= 1024 && a.keep <= 32) return run(group_kernel<T, 1, 32>, 1);
-  if (total <= 1024) return run(group_kernel<T, 4, 8>, 4);
-  if (total <= 2048 && a.keep <= 64) return run(group_kernel<T, 2, 32>, 2);
-  if (total <= 4096) return run(group_kernel<T, 4, 32>, 4);
-  return run(group_kernel<T, 8, 32>, 8);
+  const bool many = a.keep > kShortKeep;
+  if (vec) return many ? run(group_kernel<T, n, true>) : run(group_kernel<T, n, false>);
+  return many ? run(group_kernel<T, 1, true>) : run(group_kernel<T, 1, false>);
 }
 
 template <typename T>
 cudaError_t run_split(const SelectArgs& a, const SelectPlan& p, int sm_count, cudaStream_t st) {
   const int64_t rows = a.groups * a.beams, items = rows * p.segs;
+  if ((items + kRowWarps - 1) / kRowWarps > INT32_MAX) return cudaErrorInvalidConfiguration;
   SegStat* stats = static_cast<SegStat*>(a.workspace);
   Key1* cand = reinterpret_cast<Key1*>(stats + items);
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(items, static_cast<int64_t>(1) << 30));
   auto run = [&](auto fn) {
-    fn<<<grid, kSplitThreads, 0, st>>>(static_cast<const T*>(a.logits), a.group_stride, a.beam_stride, a.scores,
-                                       a.finished, rows, a.beams, a.vocab, a.keep, p.segs, cand, stats);
+    fn<<<static_cast<unsigned>((items + kRowWarps - 1) / kRowWarps), kRowWarps * kWarp, 0, st>>>(
+        static_cast<const T*>(a.logits), a.group_stride, a.beam_stride, a.scores, a.finished, rows, a.beams, a.vocab,
+        a.keep, p.segs, p.seg_tiles, cand, stats);
     return cudaGetLastError();
   };
-  cudaError_t e;
-  if (a.softmax)
-    e = p.elems == 8 ? run(split_kernel<T, 8, true>)
-                     : p.elems == 16 ? run(split_kernel<T, 16, true>) : run(split_kernel<T, 32, true>);
-  else
-    e = p.elems == 8 ? run(split_kernel<T, 8, false>)
-                     : p.elems == 16 ? run(split_kernel<T, 16, false>) : run(split_kernel<T, 32, false>);
+  const bool many = a.keep > kShortKeep;
+  const cudaError_t e = a.softmax ? many ? run(row_kernel<T, true, true>) : run(row_kernel<T, true, false>)
+                        : many    ? run(row_kernel<T, false, true>)
+                                  : run(row_kernel<T, false, false>);
   if (e != cudaSuccess) return e;
   // the join may be set up while the last segments still run; it waits for
   // them itself
@@ -944,8 +1075,8 @@ cudaError_t run_split(const SelectArgs& a, const SelectPlan& p, int sm_count, cu
 
 template <typename T>
 cudaError_t run_select(const SelectArgs& a, int sm_count, cudaStream_t st) {
-  const SelectPlan p = plan_select(a.beams, a.vocab, a.dtype);
-  return p.split ? run_split<T>(a, p, sm_count, st) : run_group<T>(a, sm_count, st);
+  const SelectPlan p = plan_select(a.groups, a.beams, a.vocab, a.dtype, a.softmax != 0);
+  return p.split ? run_split<T>(a, p, sm_count, st) : run_group<T>(a, st);
 }
 
 }  // namespace

@@ -419,11 +419,11 @@ int gann_matmul_i8(const int8_t* d_a, int64_t m, int64_t a_stride, const float* 
  *             below float32's range is written as -inf.
  * 1 <= beams, keep <= 128; beams * vocab < 2^31; groups < 2^31.
  * gann_beam_select_workspace gives the bytes of device memory that a call of
- * these sizes and type needs (0: workspace may be NULL; else 16-byte aligned). The workspace needs no
+ * these sizes, type and mode needs (0: workspace may be NULL; else 16-byte aligned). The workspace needs no
  * initialisation; calls that may overlap need one each. Device buffers on
  * `device`, enqueued on `stream`; no allocation. */
 int gann_beam_select_workspace(int64_t groups, int32_t beams, int32_t vocab, int32_t keep, int32_t dtype,
-                               int64_t* bytes);
+                               int32_t log_softmax, int64_t* bytes);
 int gann_beam_select(const void* d_logits, int32_t dtype, int64_t group_stride, int64_t beam_stride,
                      const float* d_scores, const uint8_t* d_finished, int64_t groups, int32_t beams, int32_t vocab,
                      int32_t keep, int32_t log_softmax, int32_t end_token, float* d_out_scores,

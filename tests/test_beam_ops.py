@@ -411,9 +411,9 @@ def test_c_entries_refuse_before_touching_the_gpu():
     two = C.c_int64 * 2
     bad = [sel(dt=0), sel(gs=-1), sel(bs=-1), sel(sc=None), sel(g=-1), sel(w=0), sel(w=129), sel(v=0), sel(k=0),
            sel(k=129), sel(w=128, v=2 ** 24), sel(fin=p, end=8), sel(fin=p, end=-1), sel(lg=None), sel(lg=p + 2),
-           sel(out=None), sel(out=p + 1), lib.gann_beam_select_workspace(1, 1, 8, 1, api.F32, None),
-           lib.gann_beam_select_workspace(1, 0, 8, 1, api.F32, C.byref(need)),
-           lib.gann_beam_select_workspace(1, 1, 8, 1, 0, C.byref(need)), sel(v=20000, g=999),
+           sel(out=None), sel(out=p + 1), lib.gann_beam_select_workspace(1, 1, 8, 1, api.F32, 0, None),
+           lib.gann_beam_select_workspace(1, 0, 8, 1, api.F32, 0, C.byref(need)),
+           lib.gann_beam_select_workspace(1, 1, 8, 1, 0, 0, C.byref(need)), sel(v=20000, g=999),
            reo(n=-1), reo(g=-1), reo(w=0), reo(w=129), reo(k=0), reo(k=129), reo(par=None), reo(par=p + 2),
            reo(src=None), reo(dst=None), reo(row_bytes=-1), reo(size=two(-1, 1)), reo(size=two(2 ** 40, 2 ** 40)),
            reo(dst=p, k=3, w=2), reo(dst=p, dst_beam=16), reo(dst=p, dst_stride=two(0, 8))]
