@@ -413,8 +413,8 @@ __global__ void __launch_bounds__(kRowWarps* kWarp, 5) row_kernel(const T* __res
 }
 
 // ------------------------------------------------------------ whole groups
-// Many groups, no softmax: a warp takes a whole group, in tiles of 32 (16)
-// elements a lane in registers, vectors of 16 bytes (single elements when rows
+// Many groups, no softmax: a warp takes a whole group, in tiles of 16 to
+// 64 elements a lane in registers, vectors of 16 bytes (single elements when rows
 // are not whole vectors). f = fl32(x + S_b) orders candidates as their 64-bit
 // values do, up to equality. The first tile sets a threshold of f: the keep-th
 // largest of the lanes' maxima (keep <= 16), or one bisected until between
@@ -438,12 +438,13 @@ struct Vec<T, 1> {
   __device__ __forceinline__ float max() const { return v; }
 };
 
-template <typename T, int VW, bool LONG>
-__global__ void __launch_bounds__(kGroupWarps* kWarp, LONG ? 4 : 6) group_kernel(
+template <typename T, int VW, int ELEMS, bool LONG>
+__global__ void __launch_bounds__(kGroupWarps* kWarp, LONG || ELEMS > 32 ? 4 : 6) group_kernel(
     const T* __restrict__ logits, int64_t gstride, int64_t bstride, const float* __restrict__ scores,
     const uint8_t* __restrict__ finished, int64_t groups, int beams, int vocab, int keep, int end_token, uint32_t magic,
     int shift, float* __restrict__ out_s, int32_t* __restrict__ out_p, int32_t* __restrict__ out_t) {
-  constexpr int NV = VW == 1 ? 16 : 32 / VW, kCap = Held<LONG>::value;
+  constexpr int NV = ELEMS / VW, kCap = Held<LONG>::value;
+  using Mark = typename std::conditional<(ELEMS > 32), unsigned long long, uint32_t>::type;
   __shared__ Key2 lists[kGroupWarps][kCap];
   __shared__ float cs[kGroupWarps][kBeamMax];
   const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
@@ -551,14 +552,14 @@ __global__ void __launch_bounds__(kGroupWarps* kWarp, LONG ? 4 : 6) group_kernel
         thr = lo;
       }
     }
-    uint32_t mark = 0;
+    Mark mark = 0;
     const float below = thr - fabsf(thr) * 0x1p-23f;   // by half a step of thr at least
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const float least = __fadd_rd(below, -cb[i]);
 #pragma unroll
       for (int j = 0; j < VW; ++j)
-        if (raw[i].at(j) >= least) mark |= 1u << (i * VW + j);
+        if (raw[i].at(j) >= least) mark |= Mark(1) << (i * VW + j);
     }
     int b0 = 0;
     while (true) {
@@ -567,7 +568,7 @@ __global__ void __launch_bounds__(kGroupWarps* kWarp, LONG ? 4 : 6) group_kernel
       uint32_t id = 0;
       if (__any_sync(kFull, take)) {
         if (take) {
-          const int e = __ffs(mark) - 1;
+          const int e = (ELEMS > 32 ? __ffsll(mark) : __ffs(static_cast<uint32_t>(mark))) - 1;
           id = (t0 + (e / VW) * kWarp + lane) * VW + e % VW;
           const uint32_t b = row_of(id / VW);
           const float x = Raw<T>::one(base + b * bstride + (id - b * vocab));
@@ -1036,8 +1037,11 @@ cudaError_t run_group(const SelectArgs& a, cudaStream_t st) {
     return cudaGetLastError();
   };
   const bool many = a.keep > kShortKeep;
-  if (vec) return many ? run(group_kernel<T, n, true>) : run(group_kernel<T, n, false>);
-  return many ? run(group_kernel<T, 1, true>) : run(group_kernel<T, 1, false>);
+  if (!vec) return many ? run(group_kernel<T, 1, 16, true>) : run(group_kernel<T, 1, 16, false>);
+  if (many) return run(group_kernel<T, n, 32, true>);
+  const int64_t total = static_cast<int64_t>(a.beams) * a.vocab;
+  return total > 32 * kWarp && total <= 64 * kWarp ? run(group_kernel<T, n, 64, false>)
+                                                    : run(group_kernel<T, n, 32, false>);
 }
 
 template <typename T>
