@@ -6,6 +6,7 @@
 #include <algorithm>
 #include <cstdint>
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -91,15 +92,6 @@ __global__ void __launch_bounds__(256) quantize_kernel(const uint8_t* __restrict
   }
 }
 
-// 16 bytes of a row from column b, zero past k.
-__device__ __forceinline__ uint4 load16(const int8_t* row, int b, int k) {
-  if (b + 16 <= k) return __ldg(reinterpret_cast<const uint4*>(row + b));
-  uint32_t w[4] = {0, 0, 0, 0};
-  for (int i = 0; i < 16 && b + i < k; ++i)
-    w[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(row[b + i])) << (8 * (i & 3));
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 // y = acc sa sb (+ bias): the sum is an exact integer; it is rounded to 24
 // bits when it needs more, then once at each product and sum.
 __device__ __forceinline__ float i8_value(int acc, float sa, float sb, bool has_bias, float bias) {
@@ -107,48 +99,355 @@ __device__ __forceinline__ float i8_value(int acc, float sa, float sb, bool has_
   return has_bias ? __fmaf_rn(y, sb, bias) : y * sb;
 }
 
-constexpr int kMmTile = 64;
-constexpr int kMmRow = 64 + 16;
+// ------------------------------------------------------- tensor-core product
+// The 5th-generation tensor cores multiply signed bytes with 32-bit sums
+// (tcgen05.mma, kind::i8): 128 rows of b by `tn` rows of a, 128 bytes of k a
+// step. b is the side with the 128 TMEM lanes, so a lane's results lie in one
+// column of the output and 32 lanes store 32 neighbours of an output row: any
+// output alignment is coalesced without staging. A persistent block per SM:
+//   warp 0      TMA loads of both sides' 128-byte columns into a ring of stages
+//   warp 1      issues the products; sums in TMEM, two buffers of tn columns
+//   warps 2-9   read a finished buffer, scale and store it while the next fills
+// Rows and columns past the matrices are zeros (TMA fills them), k need not be
+// a multiple of anything; tn shrinks to the rows of a that are left.
+// With few tiles and a long k, the blocks of a cluster share a tile: each sums
+// a part of k, then each gets the others' sums of a part of the columns
+// through distributed shared memory (integers: the order does not matter).
+//
+// Every wait ends: after kWaitNs the block gives up, and the tiles it has not
+// finished are filled with NaN.
+constexpr int kMmaWarps = 10, kMmaThreads = kMmaWarps * kWarp, kEpiThreads = 8 * kWarp;
+constexpr int kMmaRows = 128, kMmaK = 128;
+constexpr int kMmaMaxTn = 256, kMmaMaxStages = 12;
+constexpr uint64_t kWaitNs = 4000000000ull;
 
-// A 64 x 64 tile a CTA, 4 x 4 products a thread by dp4a.
-template <typename T>
-__global__ void __launch_bounds__(256) matmul_tile_kernel(
-    const int8_t* __restrict__ a, int64_t m, int64_t as, const float* __restrict__ sa, const int8_t* __restrict__ b,
-    int64_t n, int64_t bs, const float* __restrict__ sb, const float* __restrict__ bias, int k, T* __restrict__ out,
-    int64_t os, int64_t ntn) {
-  __shared__ __align__(16) int8_t ta[kMmTile * kMmRow], tb[kMmTile * kMmRow];
-  const int64_t i0 = (blockIdx.x / ntn) * kMmTile, j0 = (blockIdx.x % ntn) * kMmTile;
-  const int tid = threadIdx.x, lr = tid >> 2, lc = (tid & 3) * 16, tx = tid & 15, ty = tid >> 4;
-  int acc[4][4] = {};
-  for (int c = 0; c < k; c += 64) {
-    const uint4 z = make_uint4(0, 0, 0, 0);
-    const uint4 va = i0 + lr < m ? load16(a + (i0 + lr) * as, c + lc, k) : z;
-    const uint4 vb = j0 + lr < n ? load16(b + (j0 + lr) * bs, c + lc, k) : z;
-    __syncthreads();
-    *reinterpret_cast<uint4*>(ta + lr * kMmRow + lc) = va;
-    *reinterpret_cast<uint4*>(tb + lr * kMmRow + lc) = vb;
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < 16; ++q) {
-      int x[4], y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const int*>(ta + (ty + 16 * i) * kMmRow + 4 * q);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const int*>(tb + (tx + 16 * j) * kMmRow + 4 * q);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(x[i], y[j], acc[i][j]);
+struct MmaArgs {
+  const float* sa;
+  const float* sb;
+  const float* bias;
+  void* out;
+  int64_t m, n, os;
+  int k, tn, stages, split;
+  int tiles_m, tiles_n, group_m;
+};
+
+struct MmaShared {
+  uint64_t full[kMmaMaxStages], empty[kMmaMaxStages];
+  uint64_t sum_full[2], sum_empty[2], drain;
+  uint32_t tmem, dead;
+  float sa[2][kMmaMaxTn];
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void mbar_init(uint64_t* b, int n) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(n) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint64_t* b, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n.reg .pred p;\n"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(b)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ uint64_t now_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+// False when the block has given up.
+__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, uint32_t* dead) {
+  if (mbar_try(b, parity)) return true;
+  const uint64_t t0 = now_ns();
+  while (true) {
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try(b, parity)) return true;
+    if (*reinterpret_cast<volatile uint32_t*>(dead)) return false;
+    if (now_ns() - t0 > kWaitNs) {
+      *reinterpret_cast<volatile uint32_t*>(dead) = 1;
+      return false;
     }
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t r = i0 + ty + 16 * i, c = j0 + tx + 16 * j;
-      if (r < m && c < n)
-        out[r * os + c] = from_f32<T>(i8_value(acc[i][j], sa[r], sb[c], bias != nullptr, bias ? bias[c] : 0.f));
+}
+__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
+}
+// Operand tile of rows of 128 bytes, 128-byte swizzle: groups of 8 rows are
+// 1024 bytes apart.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
+  return static_cast<uint64_t>((addr & 0x3ffffu) >> 4) | (1ull << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+// s32 += s8 x s8, both operands K-major, M = 128.
+__device__ __forceinline__ uint32_t i8_instr(int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kMmaRows >> 4) << 24);
+}
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add) {
+  asm volatile(
+      "{\n.reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(instr), "r"(static_cast<uint32_t>(add))
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_load16(uint32_t addr, int (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory"); }
+
+// Tiles in groups of group_m rows of tiles: within a group the tiles that
+// share rows of b come one after another, and a's rows of the group stay in L2.
+__device__ __forceinline__ void tile_at(const MmaArgs& p, int64_t t, int& im, int& in) {
+  const int64_t per = static_cast<int64_t>(p.group_m) * p.tiles_n;
+  const int gi = static_cast<int>(t / per);
+  const int m0 = gi * p.group_m, gm = min(p.tiles_m - m0, p.group_m);
+  const int64_t r = t - gi * per;
+  in = static_cast<int>(r / gm);
+  im = m0 + static_cast<int>(r - static_cast<int64_t>(in) * gm);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kMmaThreads, 1) mma_kernel(const __grid_constant__ CUtensorMap map_a,
+                                                             const __grid_constant__ CUtensorMap map_b,
+                                                             const __grid_constant__ MmaArgs p) {
+  extern __shared__ uint8_t dyn[];
+  __shared__ MmaShared sh;
+  uint8_t* ring = dyn + (1024 - smem_u32(dyn) % 1024) % 1024;
+  const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
+  const int tile_bytes = p.tn * kMmaK, stage_bytes = kMmaRows * kMmaK + tile_bytes;
+  const int steps = (p.k + kMmaK - 1) / kMmaK;
+  const int rank = static_cast<int>(blockIdx.x) % p.split;
+  const int k0 = static_cast<int>(static_cast<int64_t>(steps) * rank / p.split);
+  const int k1 = static_cast<int>(static_cast<int64_t>(steps) * (rank + 1) / p.split);
+  const int64_t total = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
+  const int64_t t0 = blockIdx.x / p.split, dt = gridDim.x / p.split;
+  int columns = 32;   // TMEM columns: two buffers, a power of two
+  while (columns < 2 * p.tn) columns <<= 1;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int i = 0; i < p.stages; ++i) {
+        mbar_init(&sh.full[i], 1);
+        mbar_init(&sh.empty[i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&sh.sum_full[i], 1);
+        mbar_init(&sh.sum_empty[i], 8);
+      }
+      mbar_init(&sh.drain, 1);
+      sh.dead = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
+  } else if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
+                 "r"(columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tmem_fence_before();
+  }
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int s = 0, issued = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int64_t t = t0; t < total && ok; t += dt) {
+        int im, in;
+        tile_at(p, t, im, in);
+        for (int kb = k0; kb < k1; ++kb) {
+          if (!mbar_wait(&sh.empty[s], phase ^ 1u, &sh.dead)) {
+            ok = false;
+            break;
+          }
+          uint8_t* dst = ring + s * stage_bytes;
+          mbar_expect(&sh.full[s], stage_bytes);
+          tma_load(dst, &map_b, kb * kMmaK, in * kMmaRows, &sh.full[s]);
+          tma_load(dst + kMmaRows * kMmaK, &map_a, kb * kMmaK, im * p.tn, &sh.full[s]);
+          issued = min(issued + 1, p.stages);
+          if (++s == p.stages) {
+            s = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // on giving up, copies may still be in flight: see each stage's last one
+      // through (a stage whose copy was consumed long ago has passed its phase)
+      if (!ok)
+        for (int i = 0; i < issued; ++i) {
+          const int st = (s - 1 - i + 2 * p.stages) % p.stages;
+          const uint32_t ph = st < s ? phase : phase ^ 1u;
+          const uint64_t w0 = now_ns();
+          while (!mbar_try(&sh.full[st], ph) && now_ns() - w0 < kWaitNs) {
+          }
+        }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int s = 0, it = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int64_t t = t0; t < total && ok; t += dt, ++it) {
+        int im, in;
+        tile_at(p, t, im, in);
+        const int left = static_cast<int>(min(static_cast<int64_t>(p.tn), p.m - static_cast<int64_t>(im) * p.tn));
+        const uint32_t instr = i8_instr((left + 15) / 16 * 16);
+        const uint32_t d = tmem + static_cast<uint32_t>((it & 1) * p.tn);
+        if (!mbar_wait(&sh.sum_empty[it & 1], ((it >> 1) & 1) ^ 1u, &sh.dead)) {
+          ok = false;
+          break;
+        }
+        tmem_fence_after();
+        for (int kb = k0; kb < k1; ++kb) {
+          if (!mbar_wait(&sh.full[s], phase, &sh.dead)) {
+            ok = false;
+            break;
+          }
+          tmem_fence_after();
+          const uint32_t at = smem_u32(ring + s * stage_bytes);
+          const uint64_t db = operand_desc(at), da = operand_desc(at + kMmaRows * kMmaK);
+#pragma unroll
+          for (int q = 0; q < kMmaK / 32; ++q)   // 32 bytes of k an instruction
+            if (kb * kMmaK + q * 32 < p.k) mma_i8(d, db + 2 * q, da + 2 * q, instr, kb > k0 || q > 0);
+          mma_commit(&sh.empty[s]);
+          if (++s == p.stages) {
+            s = 0;
+            phase ^= 1u;
+          }
+        }
+        if (ok) mma_commit(&sh.sum_full[it & 1]);
+      }
+      if (!ok) {   // products that are still running
+        mma_commit(&sh.drain);
+        const uint64_t w0 = now_ns();
+        while (!mbar_try(&sh.drain, 0) && now_ns() - w0 < kWaitNs) {
+        }
+      }
+    }
+  } else if (p.split == 1) {
+    const int quarter = warp % 4, half = (warp - 2) / 4, etid = tid - 2 * kWarp;
+    const int cols = max(p.tn / 2, 16), c0 = half * cols;
+    int it = 0;
+    for (int64_t t = t0; t < total; t += dt, ++it) {
+      int im, in;
+      tile_at(p, t, im, in);
+      const int64_t m0 = static_cast<int64_t>(im) * p.tn;
+      const int64_t nn = static_cast<int64_t>(in) * kMmaRows + quarter * kWarp + lane;
+      const int buf = it & 1;
+      if (etid < p.tn) sh.sa[buf][etid] = m0 + etid < p.m ? p.sa[m0 + etid] : 0.f;
+      const bool inside = nn < p.n;
+      const float sb = inside ? p.sb[nn] : 0.f, bias = inside && p.bias ? p.bias[nn] : 0.f;
+      epilogue_sync();
+      const bool ok = mbar_wait(&sh.sum_full[buf], (it >> 1) & 1, &sh.dead);
+      __syncwarp();
+      tmem_fence_after();
+      const uint32_t at = tmem + (static_cast<uint32_t>(quarter * kWarp) << 16) + static_cast<uint32_t>(buf * p.tn + c0);
+      T* o = static_cast<T*>(p.out) + (m0 + c0) * p.os + nn;
+      const int end = static_cast<int>(min(static_cast<int64_t>(c0 + cols), min(static_cast<int64_t>(p.tn), p.m - m0)));
+      for (int c = c0; c < end; c += 16) {
+        int acc[16];
+        tmem_load16(at + (c - c0), acc);
+        tmem_wait_load();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          if (c + j < end && inside) {
+            const float y = i8_value(acc[j], sh.sa[buf][c + j], sb, p.bias != nullptr, bias);
+            o[static_cast<int64_t>(c - c0 + j) * p.os] = from_f32<T>(ok ? y : __int_as_float(0x7fc00000));
+          }
+        }
+      }
+      tmem_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.sum_empty[buf]);
+    }
+  } else {
+    mbar_wait(&sh.sum_full[0], 0, &sh.dead);
+  }
+
+  if (p.split > 1) {
+    // one tile a cluster; this block has summed its part of k
+    __syncwarp();
+    tmem_fence_after();
+    cluster_sync();   // no block's ring is in use any more
+    int im, in;
+    tile_at(p, t0, im, in);
+    const int64_t m0 = static_cast<int64_t>(im) * p.tn;
+    const int share = p.tn / p.split;   // columns of each block
+    if (warp >= 2) {
+      const int quarter = warp % 4, half = (warp - 2) / 4;
+      const int cols = max(p.tn / 2, 16);
+      const uint32_t at = tmem + (static_cast<uint32_t>(quarter * kWarp) << 16);
+      for (int c = half * cols; c < min(p.tn, (half + 1) * cols); c += 16) {
+        int acc[16];
+        tmem_load16(at + c, acc);
+        tmem_wait_load();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int owner = (c + j) / share, slot = rank * share + (c + j) % share;
+          const uint32_t local = smem_u32(ring) + static_cast<uint32_t>((slot * kMmaRows + quarter * kWarp + lane) * 4);
+          uint32_t remote;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(owner));
+          asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(remote), "r"(acc[j]) : "memory");
+        }
+      }
+    }
+    uint32_t bad = *reinterpret_cast<volatile uint32_t*>(&sh.dead);
+    cluster_sync();
+    // a block that gave up has spoilt the sums of all of them
+    for (int r = 0; r < p.split; ++r) {
+      uint32_t remote, v;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(&sh.dead)), "r"(r));
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
+      bad |= v;
+    }
+    const int* recv = reinterpret_cast<const int*>(ring);
+    for (int e = tid; e < share * kMmaRows; e += kMmaThreads) {
+      const int c = e / kMmaRows, r = e % kMmaRows;
+      const int64_t mm = m0 + rank * share + c, nn = static_cast<int64_t>(in) * kMmaRows + r;
+      if (mm >= p.m || nn >= p.n) continue;
+      int acc = 0;
+      for (int q = 0; q < p.split; ++q) acc += recv[(q * share + c) * kMmaRows + r];
+      const float y = i8_value(acc, p.sa[mm], p.sb[nn], p.bias != nullptr, p.bias ? p.bias[nn] : 0.f);
+      static_cast<T*>(p.out)[mm * p.os + nn] = from_f32<T>(bad ? __int_as_float(0x7fc00000) : y);
+    }
+    cluster_sync();   // the flags of this block are not read any more
+  }
+  tmem_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tmem_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+  }
 }
 
 }  // namespace
@@ -166,19 +465,109 @@ cudaError_t launch_quantize_rows(const void* x, int64_t rows, int64_t stride, in
   return run(quantize_kernel<__nv_bfloat16>);
 }
 
+namespace {
+
+// cuTensorMapEncodeTiled from the driver that the runtime has loaded.
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeTiled>(f);
+  }();
+  return fn;
+}
+
+// Rows of k bytes in boxes of 128 bytes by `box` rows, zeros outside.
+cudaError_t encode_rows(CUtensorMap* map, const int8_t* p, int64_t rows, int64_t stride, int k, int box) {
+  const EncodeTiled fn = encode_tiled();
+  if (!fn) return cudaErrorNotSupported;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride)};
+  const cuuint32_t boxes[2] = {kMmaK, static_cast<cuuint32_t>(box)};
+  const cuuint32_t steps[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(p), dims, strides, boxes, steps,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+struct MmaPlan {
+  int tn, split;
+};
+
+// Rows of a in a tile: all of them up to 256, in steps that the two output
+// halves share; with more, 256, halved while the tiles do not fill the GPU.
+// A tile's k is split over 2, 4 or 8 blocks while blocks are idle and each
+// part keeps four steps of 128.
+MmaPlan plan_mma(int64_t m, int64_t n, int k, int sm_count) {
+  MmaPlan p{16, 1};
+  while (p.tn < m && p.tn < kMmaMaxTn) p.tn <<= 1;
+  const int64_t tn_tiles = (n + kMmaRows - 1) / kMmaRows;
+  while (m > p.tn / 2 && p.tn > 64 && tn_tiles * ((m + p.tn - 1) / p.tn) * 2 <= sm_count) p.tn >>= 1;
+  const int64_t tiles = tn_tiles * ((m + p.tn - 1) / p.tn);
+  const int steps = (k + kMmaK - 1) / kMmaK;
+  while (p.split < 8 && tiles * p.split * 2 <= sm_count && steps >= p.split * 8) p.split <<= 1;
+  return p;
+}
+
+}  // namespace
+
 cudaError_t launch_matmul_i8(const int8_t* a, int64_t m, int64_t as, const float* sa, const int8_t* b, int64_t n,
                              int64_t bs, const float* sb, const float* bias, int k, void* out, int64_t os, int dtype,
                              int sm_count, cudaStream_t st) {
   if (m <= 0 || n <= 0) return cudaSuccess;
-  const int64_t ntm = (m + kMmTile - 1) / kMmTile, ntn = (n + kMmTile - 1) / kMmTile;
-  if (ntm * ntn > INT32_MAX) return cudaErrorInvalidConfiguration;
-  auto run = [&](auto fn, auto* o) {
-    fn<<<static_cast<unsigned>(ntm * ntn), 256, 0, st>>>(a, m, as, sa, b, n, bs, sb, bias, k, o, os, ntn);
-    return cudaGetLastError();
+  const MmaPlan plan = plan_mma(m, n, k, sm_count);
+  MmaArgs p{};
+  p.sa = sa;
+  p.sb = sb;
+  p.bias = bias;
+  p.out = out;
+  p.m = m;
+  p.n = n;
+  p.os = os;
+  p.k = k;
+  p.tn = plan.tn;
+  p.split = plan.split;
+  const int64_t tiles_m = (m + p.tn - 1) / p.tn, tiles_n = (n + kMmaRows - 1) / kMmaRows;
+  p.tiles_m = static_cast<int>(tiles_m);
+  p.tiles_n = static_cast<int>(tiles_n);
+  // rows of a that stay in L2 beside the stream of b: about 32 MB
+  p.group_m = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tiles_m, (32 << 20) / (static_cast<int64_t>(k) * p.tn + 1))));
+  const int stage = kMmaRows * kMmaK + p.tn * kMmaK;
+  p.stages = std::min({kMmaMaxStages, (200 * 1024) / stage, std::max(2, (k + kMmaK - 1) / kMmaK * 2)});
+  const size_t ring = std::max<size_t>(static_cast<size_t>(p.stages) * stage,
+                                       p.split > 1 ? static_cast<size_t>(p.tn) * kMmaRows * 4 : 0);
+  const size_t smem = ring + 1024;
+  CUtensorMap ma, mb;
+  cudaError_t e = encode_rows(&ma, a, m, as, k, p.tn);
+  if (e == cudaSuccess) e = encode_rows(&mb, b, n, bs, k, kMmaRows);
+  if (e != cudaSuccess) return e;
+  const int64_t blocks = p.split > 1 ? tiles_m * tiles_n * p.split : std::min<int64_t>(tiles_m * tiles_n, sm_count);
+  auto run = [&](auto fn) -> cudaError_t {
+    cudaError_t r = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (r != cudaSuccess) return r;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(p.split);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+    cfg.blockDim = dim3(kMmaThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, fn, ma, mb, p);
   };
-  if (dtype == GANN_F32) return run(matmul_tile_kernel<float>, static_cast<float*>(out));
-  if (dtype == GANN_F16) return run(matmul_tile_kernel<__half>, static_cast<__half*>(out));
-  return run(matmul_tile_kernel<__nv_bfloat16>, static_cast<__nv_bfloat16*>(out));
+  if (dtype == GANN_F32) return run(mma_kernel<float>);
+  if (dtype == GANN_F16) return run(mma_kernel<__half>);
+  return run(mma_kernel<__nv_bfloat16>);
 }
 
 }  // namespace gann
