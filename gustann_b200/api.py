@@ -76,6 +76,8 @@ class _Info(C.Structure):
 
 
 class _State(C.Structure):
+    """gann_state: 13 words of 8 bytes."""
+
     _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("src_group", C.c_int64), ("src_beam", C.c_int64),
                 ("src_stride", C.c_int64 * 2), ("dst_group", C.c_int64), ("dst_beam", C.c_int64),
                 ("dst_stride", C.c_int64 * 2), ("size", C.c_int64 * 2), ("row_bytes", C.c_int64)]
@@ -114,7 +116,7 @@ def _load() -> C.CDLL:
     lib.gann_beam_select_workspace.argtypes = [i64, i32, i32, i32, i32, i32, C.POINTER(i64)]
     lib.gann_beam_select.argtypes = [vp, i32, i64, i64, vp, vp, i64, i32, i32, i32, i32, i32, vp, vp, vp, vp, i64,
                                      i32, vp]
-    lib.gann_reorder_states.argtypes = [C.POINTER(_State), i32, vp, i64, i32, i32, i32, vp]
+    lib.gann_reorder_states.argtypes = [vp, i32, vp, i64, i32, i32, i32, vp]
     for name in EXPORTS:
         if name != "gann_last_error":
             getattr(lib, name).restype = C.c_int
@@ -453,44 +455,43 @@ def _fail(msg: str):
     raise GustANNError(GANN_EINVAL, msg)
 
 
+_torch = None
+_FLOATS = {}   # torch dtype -> gann_float
+
+
+def _get_torch():
+    """torch, imported with the first call that takes tensors."""
+    global _torch
+    if _torch is None:
+        import torch
+        _FLOATS.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+        _torch = torch
+    return _torch
+
+
 def _float_code(dtype, who: str) -> int:
-    import torch
-    code = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(dtype)
+    code = _FLOATS.get(dtype)
     if code is None:
         _fail(f"{who}: dtype must be float32, float16 or bfloat16")
     return code
 
 
 def _on_cuda(who: str, *tensors):
+    """The tensors' common device and its index."""
     dev = tensors[0].device
     for t in tensors:
-        if not t.is_cuda or t.device != dev:
+        if t.device != dev or not t.is_cuda:
             _fail(f"{who}: tensors must be on one CUDA device")
-    return dev
+    return dev, dev.index
 
 
-class _Stream:
-    """Outputs and workspaces of a call are allocated on the stream it runs on:
-    ``stream`` (a ``cudaStream_t``; 0 the default stream), or torch's current
-    stream of the device when it is None."""
-
-    def __init__(self, device, stream):
-        import torch
-        cur = torch.cuda.current_stream(device).cuda_stream
-        self.handle = cur if stream is None else stream
-        self._ctx = None
-        if self.handle != cur:
-            self._ctx = torch.cuda.stream(torch.cuda.ExternalStream(stream, device) if stream
-                                          else torch.cuda.default_stream(device))
-
-    def __enter__(self):
-        if self._ctx is not None:
-            self._ctx.__enter__()
-        return self.handle or None
-
-    def __exit__(self, *exc):
-        if self._ctx is not None:
-            self._ctx.__exit__(*exc)
+def _stream_scope(device, stream: int):
+    """Makes ``stream`` (a ``cudaStream_t``, 0 the default stream) torch's
+    current one, so that a call's outputs and workspaces are allocated on the
+    stream it runs on."""
+    torch = _get_torch()
+    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device) if stream
+                             else torch.cuda.default_stream(device))
 
 
 def _extent(t):
@@ -512,32 +513,37 @@ def quantize_rows(x, stream: int | None = None):
     boundaries, as :func:`matmul_i8` wants them. A row with a NaN or an
     infinity gets scale NaN and codes 0. ``stream``: a ``cudaStream_t``, or
     None for torch's current stream."""
-    import torch
+    torch = _get_torch()
     if x.dim() != 2:
         _fail("quantize_rows: x must have two dimensions")
     dt = _float_code(x.dtype, "quantize_rows")
-    dev = _on_cuda("quantize_rows", x)
+    dev, index = _on_cuda("quantize_rows", x)
     n, d = x.shape
-    if d > 1 and x.stride(1) != 1:
+    step, inner = x.stride()
+    if inner != 1 and d > 1:
         _fail("quantize_rows: rows must be contiguous")
-    with _Stream(dev, stream) as st:
-        codes = torch.empty((n, (d + 15) // 16 * 16), dtype=torch.int8, device=dev)
-        scales = torch.empty(n, dtype=torch.float32, device=dev)
-        _check(lib.gann_quantize_rows(x.data_ptr(), n, x.stride(0) * x.element_size(), d, dt, codes.data_ptr(),
-                                      codes.stride(0), scales.data_ptr(), dev.index or 0, st))
-    return codes[:, :d], scales
+    if stream is not None:
+        with _stream_scope(dev, stream):
+            return quantize_rows(x)
+    pad = (d + 15) // 16 * 16
+    codes = torch.empty_strided((n, d), (pad, 1), dtype=torch.int8, device=dev)
+    scales = torch.empty(n, dtype=torch.float32, device=dev)
+    _check(lib.gann_quantize_rows(x.data_ptr(), n, step * x.element_size(), d, dt, codes.data_ptr(), pad,
+                                  scales.data_ptr(), index, torch._C._cuda_getCurrentRawStream(index)))
+    return codes, scales
 
 
 def _i8_rows(name: str, codes, scales):
-    import torch
-    if codes.dtype != torch.int8 or codes.dim() != 2:
+    if codes.dtype != _torch.int8 or codes.dim() != 2:
         _fail(f"matmul_i8: {name} must be int8 with two dimensions")
     n, k = codes.shape
-    if scales.dtype != torch.float32 or scales.shape != (n,) or (n > 1 and scales.stride(0) != 1):
+    stride, inner = codes.stride()
+    if scales.dtype != _torch.float32 or scales.shape != (n,) or (n > 1 and scales.stride(0) != 1):
         _fail(f"matmul_i8: {name}'s scales must be contiguous float32, one a row")
-    if k > 1 and codes.stride(1) != 1:
+    if inner != 1 and k > 1:
         _fail(f"matmul_i8: rows of {name} must be contiguous")
-    stride = codes.stride(0) if n > 1 else (k + 15) // 16 * 16
+    if n <= 1:
+        stride = (k + 15) // 16 * 16
     if n and (stride % 16 or codes.data_ptr() % 16):
         _fail(f"matmul_i8: rows of {name} must start on 16-byte boundaries, as quantize_rows lays them out")
     return n, k, stride
@@ -552,7 +558,7 @@ def matmul_i8(a, a_scales, b, b_scales, bias=None, dtype=None, out=None, stream:
     bfloat16 too), or fills ``out`` when it is given (contiguous rows).
     Queries against base rows: their scores; tokens against the rows of a
     weight matrix: a linear layer. ``stream`` as in :func:`quantize_rows`."""
-    import torch
+    torch = _get_torch()
     m, k, sa = _i8_rows("a", a, a_scales)
     n, kb, sb = _i8_rows("b", b, b_scales)
     if k != kb:
@@ -562,7 +568,7 @@ def matmul_i8(a, a_scales, b, b_scales, bias=None, dtype=None, out=None, stream:
         if bias.dtype != torch.float32 or bias.shape != (n,) or (n > 1 and bias.stride(0) != 1):
             _fail("matmul_i8: bias must be contiguous float32, one a row of b")
         ins.append(bias)
-    dev = _on_cuda("matmul_i8", *ins)
+    dev, index = _on_cuda("matmul_i8", *ins)
     if out is not None:
         _on_cuda("matmul_i8", a, out)
         if out.shape != (m, n) or (dtype is not None and out.dtype != dtype):
@@ -571,13 +577,18 @@ def matmul_i8(a, a_scales, b, b_scales, bias=None, dtype=None, out=None, stream:
             _fail("matmul_i8: rows of out must be contiguous and apart from each other")
         if not all(_disjoint(out, t) for t in ins):
             _fail("matmul_i8: out overlaps an input")
-    dt = _float_code(out.dtype if out is not None else dtype or torch.float32, "matmul_i8")
-    with _Stream(dev, stream) as st:
-        if out is None:
-            out = torch.empty((m, n), dtype=dtype or torch.float32, device=dev)
-        _check(lib.gann_matmul_i8(a.data_ptr(), m, sa, a_scales.data_ptr(), b.data_ptr(), n, sb, b_scales.data_ptr(),
-                                  None if bias is None else bias.data_ptr(), k, out.data_ptr(),
-                                  out.stride(0) if m > 1 else n, dt, dev.index or 0, st))
+        dtype = out.dtype
+    elif dtype is None:
+        dtype = torch.float32
+    dt = _float_code(dtype, "matmul_i8")
+    if stream is not None:
+        with _stream_scope(dev, stream):
+            return matmul_i8(a, a_scales, b, b_scales, bias, dtype, out)
+    if out is None:
+        out = torch.empty(m, n, dtype=dtype, device=dev)
+    _check(lib.gann_matmul_i8(a.data_ptr(), m, sa, a_scales.data_ptr(), b.data_ptr(), n, sb, b_scales.data_ptr(),
+                              None if bias is None else bias.data_ptr(), k, out.data_ptr(),
+                              out.stride(0) if m > 1 else n, dt, index, torch._C._cuda_getCurrentRawStream(index)))
     return out
 
 
@@ -593,34 +604,38 @@ def beam_select(scores, logits, k: int, log_softmax: bool = False, finished=None
     beam has one candidate, ``end_token`` at its own score. Returns ``(scores
     float32, parents int32, tokens int32)``, each [g, k], filled up with
     -inf, -1, -1. w and k at most 128. ``stream`` as in :func:`quantize_rows`."""
-    import torch
+    torch = _get_torch()
     if logits.dim() != 3 or scores.dtype != torch.float32 or scores.shape != logits.shape[:2]:
         _fail("beam_select: need logits [g, w, v] and float32 scores [g, w]")
     dt = _float_code(logits.dtype, "beam_select")
     g, w, v = logits.shape
-    ins = [scores, logits]
-    if finished is not None:
+    if finished is None:
+        dev, index = _on_cuda("beam_select", scores, logits)
+    else:
         if finished.dtype not in (torch.bool, torch.uint8) or finished.shape != (g, w):
             _fail("beam_select: finished must be bool [g, w]")
-        ins.append(finished)
-    dev = _on_cuda("beam_select", *ins)
-    if v > 1 and logits.stride(2) != 1:
+        dev, index = _on_cuda("beam_select", scores, logits, finished)
+    gs, bs, inner = logits.stride()
+    if inner != 1 and v > 1:
         _fail("beam_select: the last dimension of logits must be contiguous")
-    with _Stream(dev, stream) as st:
-        scores = scores.contiguous()
-        if finished is not None:
-            finished = finished.contiguous()
-        need = C.c_int64()
-        _check(lib.gann_beam_select_workspace(g, w, v, k, dt, int(bool(log_softmax)), C.byref(need)))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
-        out_s = torch.empty((g, k), dtype=torch.float32, device=dev)
-        out_p = torch.empty((g, k), dtype=torch.int32, device=dev)
-        out_t = torch.empty((g, k), dtype=torch.int32, device=dev)
-        _check(lib.gann_beam_select(logits.data_ptr(), dt, logits.stride(0), logits.stride(1), scores.data_ptr(),
-                                    None if finished is None else finished.data_ptr(), g, w, v, k,
-                                    int(bool(log_softmax)), end_token, out_s.data_ptr(), out_p.data_ptr(),
-                                    out_t.data_ptr(), None if ws is None else ws.data_ptr(), need.value,
-                                    dev.index or 0, st))
+    if stream is not None:
+        with _stream_scope(dev, stream):
+            return beam_select(scores, logits, k, log_softmax, finished, end_token)
+    soft = 1 if log_softmax else 0
+    need = C.c_int64()
+    _check(lib.gann_beam_select_workspace(g, w, v, k, dt, soft, C.byref(need)))
+    scores = scores.contiguous()
+    if finished is not None:
+        finished = finished.contiguous()
+    ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
+    out_s = torch.empty(g, k, dtype=torch.float32, device=dev)
+    out_p = torch.empty(g, k, dtype=torch.int32, device=dev)
+    out_t = torch.empty_like(out_p)
+    _check(lib.gann_beam_select(logits.data_ptr(), dt, gs, bs, scores.data_ptr(),
+                                None if finished is None else finished.data_ptr(), g, w, v, k, soft, end_token,
+                                out_s.data_ptr(), out_p.data_ptr(), out_t.data_ptr(),
+                                None if ws is None else ws.data_ptr(), need.value, index,
+                                torch._C._cuda_getCurrentRawStream(index)))
     return out_s, out_p, out_t
 
 
@@ -633,6 +648,8 @@ def _state_layout(src, dst):
     run = 1
     while dims and dims[-1][1] == run and dims[-1][2] == run:
         run *= dims.pop()[0]
+    if not dims:
+        return [1, 1], [0, 0], [0, 0], run * es
     merged = []
     for n, a, b in dims:
         if merged and merged[-1][1] == n * a and merged[-1][2] == n * b:
@@ -665,36 +682,38 @@ def reorder_states(states, parents, out=None, stream: int | None = None):
     ``out`` new tensors [g, k, ...] are returned; ``out`` gives the targets,
     and may be ``states`` itself: in place (k <= w; beams from k on stay as they were).
     Other overlaps are refused. ``stream`` as in :func:`quantize_rows`."""
-    import torch
+    torch = _get_torch()
     one = torch.is_tensor(states)
     srcs = [states] if one else list(states)
     if parents.dim() != 2 or parents.dtype != torch.int32:
         _fail("reorder_states: parents must be int32 [g, k]")
     g, k = parents.shape
-    dev = _on_cuda("reorder_states", parents, *srcs)
-    for s in srcs:
-        if s.dim() < 2 or s.shape[0] != g or s.shape[1] != srcs[0].shape[1]:
-            _fail("reorder_states: every state must be [g, w, ...] with the groups of parents")
+    dev, index = _on_cuda("reorder_states", parents, *srcs)
     if not srcs:
         return []
-    w = srcs[0].shape[1]
-    with _Stream(dev, stream) as st:
-        if out is None:
-            dsts = [torch.empty((g, k) + s.shape[2:], dtype=s.dtype, device=dev) for s in srcs]
-        else:
-            dsts = [out] if torch.is_tensor(out) else list(out)
-            _check_targets(srcs, dsts, parents, g, k)
-        table = (_State * len(srcs))()
-        for e, s, d in zip(table, srcs, dsts):
-            lay = _state_layout(s, d)
-            if lay is None:
-                _fail("reorder_states: a state has more than two strided dimensions behind (g, w)")
-            es = s.element_size()
-            e.src, e.dst = s.data_ptr(), d.data_ptr()
-            e.src_group, e.src_beam = s.stride(0) * es, s.stride(1) * es
-            e.dst_group, e.dst_beam = d.stride(0) * es, d.stride(1) * es
-            e.size[:], e.src_stride[:], e.dst_stride[:], e.row_bytes = lay
-        _check(lib.gann_reorder_states(table, len(srcs), parents.contiguous().data_ptr(), g, w, k, dev.index or 0, st))
+    w = srcs[0].shape[1] if srcs[0].dim() > 1 else 0
+    for s in srcs:
+        if s.dim() < 2 or s.shape[0] != g or s.shape[1] != w:
+            _fail("reorder_states: every state must be [g, w, ...] with the groups of parents")
+    if out is not None:
+        dsts = [out] if torch.is_tensor(out) else list(out)
+        _check_targets(srcs, dsts, parents, g, k)
+    if stream is not None:
+        with _stream_scope(dev, stream):
+            return reorder_states(states, parents, out)
+    if out is None:
+        dsts = [torch.empty(g, k, *s.shape[2:], dtype=s.dtype, device=dev) for s in srcs]
+    table = []
+    for s, d in zip(srcs, dsts):
+        lay = _state_layout(s, d)
+        if lay is None:
+            _fail("reorder_states: a state has more than two strided dimensions behind (g, w)")
+        size, ss, ds, row = lay
+        es, a, b = s.element_size(), s.stride(), d.stride()
+        table += [s.data_ptr(), d.data_ptr(), a[0] * es, a[1] * es, *ss, b[0] * es, b[1] * es, *ds, *size, row]
+    parents = parents.contiguous()
+    _check(lib.gann_reorder_states((C.c_int64 * len(table))(*table), len(srcs), parents.data_ptr(), g, w, k, index,
+                                   torch._C._cuda_getCurrentRawStream(index)))
     return dsts[0] if one else dsts
 
 

@@ -92,11 +92,11 @@ __global__ void __launch_bounds__(256) quantize_kernel(const uint8_t* __restrict
   }
 }
 
-// y = acc sa sb (+ bias): the sum is an exact integer; it is rounded to 24
-// bits when it needs more, then once at each product and sum.
-__device__ __forceinline__ float i8_value(int acc, float sa, float sb, bool has_bias, float bias) {
-  const float y = static_cast<float>(acc) * sa;
-  return has_bias ? __fmaf_rn(y, sb, bias) : y * sb;
+// y = acc sa sb + bias (0 when there is none): the sum is an exact integer; it
+// is rounded to 24 bits when it needs more, then after the first product and
+// after the second with its sum.
+__device__ __forceinline__ float i8_value(int acc, float sa, float sb, float bias) {
+  return __fmaf_rn(static_cast<float>(acc) * sa, sb, bias);
 }
 
 // ------------------------------------------------------- tensor-core product
@@ -127,7 +127,7 @@ struct MmaArgs {
   const float* bias;
   void* out;
   int64_t m, n, os;
-  int k, tn, stages, split;
+  int k, tn, stages, split, pairs;
   int tiles_m, tiles_n, group_m;
 };
 
@@ -135,7 +135,7 @@ struct MmaShared {
   uint64_t full[kMmaMaxStages], empty[kMmaMaxStages];
   uint64_t sum_full[2], sum_empty[2], drain;
   uint32_t tmem, dead;
-  float sa[2][kMmaMaxTn];
+  __align__(16) float sa[2][kMmaMaxTn];
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -206,12 +206,24 @@ __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint3
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void tmem_load16(uint32_t addr, int (&v)[16]) {
+__device__ __forceinline__ void tmem_load(uint32_t addr, int (&v)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
-      "[%16];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+      "%13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_load(uint32_t addr, int (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+      "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, "
+      "[%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]),
+        "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]),
+        "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]),
+        "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(addr));
 }
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -231,6 +243,45 @@ __device__ __forceinline__ void tile_at(const MmaArgs& p, int64_t t, int& im, in
   const int64_t r = t - gi * per;
   in = static_cast<int>(r / gm);
   im = m0 + static_cast<int>(r - static_cast<int64_t>(in) * gm);
+}
+
+// A warp's 32 neighbours of 32 output rows: o is the lane's element of the first.
+__device__ __forceinline__ void store_columns(float* o, int64_t os, const float (&y)[32], int, bool) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    *o = y[j];
+    o += os;
+  }
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, const __half*) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, const __nv_bfloat16*) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// 16-bit results: with rows of 4-byte multiples (pairs), lanes 2i and 2i + 1
+// trade values so that one stores both of an even row, the other both of the
+// odd one: half the stores.
+template <typename T>
+__device__ __forceinline__ void store_columns(T* o, int64_t os, const float (&y)[32], int lane, bool pairs) {
+  if (pairs) {
+    const bool odd = lane & 1;
+    T* q = odd ? o - 1 + os : o;
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      const float got = __shfl_xor_sync(kFull, odd ? y[j] : y[j + 1], 1);
+      *reinterpret_cast<uint32_t*>(q) = odd ? pack2(got, y[j + 1], q) : pack2(y[j], got, q);
+      q += 2 * os;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      *o = from_f32<T>(y[j]);
+      o += os;
+    }
+  }
 }
 
 template <typename T>
@@ -365,26 +416,47 @@ __global__ void __launch_bounds__(kMmaThreads, 1) mma_kernel(const __grid_consta
       const int64_t nn = static_cast<int64_t>(in) * kMmaRows + quarter * kWarp + lane;
       const int buf = it & 1;
       if (etid < p.tn) sh.sa[buf][etid] = m0 + etid < p.m ? p.sa[m0 + etid] : 0.f;
-      const bool inside = nn < p.n;
-      const float sb = inside ? p.sb[nn] : 0.f, bias = inside && p.bias ? p.bias[nn] : 0.f;
+      const bool inside = nn < p.n, whole = __all_sync(kFull, inside);
+      float sb = inside ? p.sb[nn] : 0.f;
+      const float bias = inside && p.bias ? p.bias[nn] : 0.f;
       epilogue_sync();
-      const bool ok = mbar_wait(&sh.sum_full[buf], (it >> 1) & 1, &sh.dead);
-      __syncwarp();
+      // a block that gave up: NaN
+      if (!__all_sync(kFull, mbar_wait(&sh.sum_full[buf], (it >> 1) & 1, &sh.dead))) sb = __int_as_float(0x7fc00000);
       tmem_fence_after();
       const uint32_t at = tmem + (static_cast<uint32_t>(quarter * kWarp) << 16) + static_cast<uint32_t>(buf * p.tn + c0);
       T* o = static_cast<T*>(p.out) + (m0 + c0) * p.os + nn;
-      const int end = static_cast<int>(min(static_cast<int64_t>(c0 + cols), min(static_cast<int64_t>(p.tn), p.m - m0)));
-      for (int c = c0; c < end; c += 16) {
+      const int end = static_cast<int>(min(static_cast<int64_t>(cols), min(static_cast<int64_t>(p.tn), p.m - m0) - c0));
+      const float* sa = sh.sa[buf] + c0;
+      int c = 0;
+      if (whole && end >= 32) {
+        // 32 columns at a time, the next 32 on their way
+        int v[32];
+        tmem_load(at, v);
+        for (; c + 32 <= end; c += 32) {
+          tmem_wait_load();
+          float y[32];
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 s4 = *reinterpret_cast<const float4*>(sa + c + j);
+            y[j] = i8_value(v[j], s4.x, sb, bias);
+            y[j + 1] = i8_value(v[j + 1], s4.y, sb, bias);
+            y[j + 2] = i8_value(v[j + 2], s4.z, sb, bias);
+            y[j + 3] = i8_value(v[j + 3], s4.w, sb, bias);
+          }
+          if (c + 64 <= end) tmem_load(at + c + 32, v);
+          store_columns(o, p.os, y, lane, p.pairs);
+          o += 32 * p.os;
+        }
+        tmem_wait_load();
+      }
+      for (; c < end; c += 16) {
         int acc[16];
-        tmem_load16(at + (c - c0), acc);
+        tmem_load(at + c, acc);
         tmem_wait_load();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          if (c + j < end && inside) {
-            const float y = i8_value(acc[j], sh.sa[buf][c + j], sb, p.bias != nullptr, bias);
-            o[static_cast<int64_t>(c - c0 + j) * p.os] = from_f32<T>(ok ? y : __int_as_float(0x7fc00000));
-          }
-        }
+        for (int j = 0; j < 16; ++j)
+          if (c + j < end && inside) o[j * p.os] = from_f32<T>(i8_value(acc[j], sa[c + j], sb, bias));
+        o += 16 * p.os;
       }
       tmem_fence_before();
       __syncwarp();
@@ -409,7 +481,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) mma_kernel(const __grid_consta
       const uint32_t at = tmem + (static_cast<uint32_t>(quarter * kWarp) << 16);
       for (int c = half * cols; c < min(p.tn, (half + 1) * cols); c += 16) {
         int acc[16];
-        tmem_load16(at + c, acc);
+        tmem_load(at + c, acc);
         tmem_wait_load();
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
@@ -437,7 +509,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) mma_kernel(const __grid_consta
       if (mm >= p.m || nn >= p.n) continue;
       int acc = 0;
       for (int q = 0; q < p.split; ++q) acc += recv[(q * share + c) * kMmaRows + r];
-      const float y = i8_value(acc, p.sa[mm], p.sb[nn], p.bias != nullptr, p.bias ? p.bias[nn] : 0.f);
+      const float y = i8_value(acc, p.sa[mm], p.sb[nn], p.bias ? p.bias[nn] : 0.f);
       static_cast<T*>(p.out)[mm * p.os + nn] = from_f32<T>(bad ? __int_as_float(0x7fc00000) : y);
     }
     cluster_sync();   // the flags of this block are not read any more
@@ -534,6 +606,7 @@ cudaError_t launch_matmul_i8(const int8_t* a, int64_t m, int64_t as, const float
   p.k = k;
   p.tn = plan.tn;
   p.split = plan.split;
+  p.pairs = os % 2 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0;
   const int64_t tiles_m = (m + p.tn - 1) / p.tn, tiles_n = (n + kMmaRows - 1) / kMmaRows;
   p.tiles_m = static_cast<int>(tiles_m);
   p.tiles_n = static_cast<int>(tiles_n);
