@@ -107,19 +107,25 @@ __device__ __forceinline__ float i8_value(int acc, float sa, float sb, float bia
 // output alignment is coalesced without staging. A persistent block per SM:
 //   warp 0      TMA loads of both sides' 128-byte columns into a ring of stages
 //   warp 1      issues the products; sums in TMEM, two buffers of tn columns
-//   warps 2-9   read a finished buffer, scale and store it while the next fills
+//   the others  read a finished buffer, scale and store it while the next fills
 // Rows and columns past the matrices are zeros (TMA fills them), k need not be
 // a multiple of anything; tn shrinks to the rows of a that are left.
+// Large products use pairs of blocks (cta_group::2): 256 rows of b by tn rows of
+// a, each block loading its 128 rows of b and half of a's rows, so a step
+// moves 32 KB instead of 48 KB into an SM for the same work. The loads of a
+// step are in flight for longer than the products take, so their bytes set
+// the pace.
 // With few tiles and a long k, the blocks of a cluster share a tile: each sums
 // a part of k, then each gets the others' sums of a part of the columns
 // through distributed shared memory (integers: the order does not matter).
 //
-// Every wait ends: after kWaitNs the block gives up, and the tiles it has not
+// Every wait ends: after kWaitClocks the block gives up, and the tiles it has not
 // finished are filled with NaN.
-constexpr int kMmaWarps = 10, kMmaThreads = kMmaWarps * kWarp, kEpiThreads = 8 * kWarp;
+constexpr int kEpiWarps = 8, kEpiThreads = kEpiWarps * kWarp;
+constexpr int kMmaThreads = kEpiThreads + 2 * kWarp;
 constexpr int kMmaRows = 128, kMmaK = 128;
 constexpr int kMmaMaxTn = 256, kMmaMaxStages = 12;
-constexpr uint64_t kWaitNs = 4000000000ull;
+constexpr int64_t kWaitClocks = 8000000000ll;   // about 4 s
 
 struct MmaArgs {
   const float* sa;
@@ -159,23 +165,26 @@ __device__ __forceinline__ bool mbar_try(uint64_t* b, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ uint64_t now_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-  return t;
-}
-// False when the block has given up.
+// False when the block has given up. The clock is looked at once in 256 tries
+// (each of which the hardware may suspend for a while).
 __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, uint32_t* dead) {
-  if (mbar_try(b, parity)) return true;
-  const uint64_t t0 = now_ns();
+  for (int i = 0; i < 256; ++i)
+    if (mbar_try(b, parity)) return true;
+  const int64_t t0 = clock64();
   while (true) {
-    for (int i = 0; i < 64; ++i)
+    for (int i = 0; i < 256; ++i)
       if (mbar_try(b, parity)) return true;
     if (*reinterpret_cast<volatile uint32_t*>(dead)) return false;
-    if (now_ns() - t0 > kWaitNs) {
+    if (clock64() - t0 > kWaitClocks) {
       *reinterpret_cast<volatile uint32_t*>(dead) = 1;
       return false;
     }
+  }
+}
+// The same without a word to the others: for what is still in flight then.
+__device__ __forceinline__ void mbar_drain(uint64_t* b, uint32_t parity) {
+  const int64_t t0 = clock64();
+  while (!mbar_try(b, parity) && clock64() - t0 < kWaitClocks) {
   }
 }
 __device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
@@ -185,26 +194,64 @@ __device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int 
       "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
       : "memory");
 }
+// The same within a pair of blocks, counted by the first block's barrier.
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3}], [%4];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t in_block(const void* p, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 // Operand tile of rows of 128 bytes, 128-byte swizzle: groups of 8 rows are
 // 1024 bytes apart.
 __device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
   return static_cast<uint64_t>((addr & 0x3ffffu) >> 4) | (1ull << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
          (1ull << 46) | (2ull << 61);
 }
-// s32 += s8 x s8, both operands K-major, M = 128.
+// s32 += s8 x s8, both operands K-major.
+template <bool PAIR>
 __device__ __forceinline__ uint32_t i8_instr(int n) {
-  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kMmaRows >> 4) << 24);
+  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>((PAIR ? 2 : 1) * kMmaRows >> 4) << 24);
 }
+template <bool PAIR>
 __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add) {
-  asm volatile(
-      "{\n.reg .pred p;\n"
-      "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(instr), "r"(static_cast<uint32_t>(add))
-      : "memory");
+  if (PAIR)
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(instr), "r"(static_cast<uint32_t>(add))
+        : "memory");
+  else
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(instr), "r"(static_cast<uint32_t>(add))
+        : "memory");
 }
+// An arrival, once the products issued so far are done, at this block's
+// barrier, or at both of a pair's.
+template <bool PAIR>
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+  if (PAIR)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_load(uint32_t addr, int (&v)[16]) {
   asm volatile(
@@ -230,6 +277,7 @@ __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::l
 __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory"); }
@@ -284,7 +332,7 @@ __device__ __forceinline__ void store_columns(T* o, int64_t os, const float (&y)
   }
 }
 
-template <typename T>
+template <typename T, bool PAIR>
 __global__ void __launch_bounds__(kMmaThreads, 1) mma_kernel(const __grid_constant__ CUtensorMap map_a,
                                                              const __grid_constant__ CUtensorMap map_b,
                                                              const __grid_constant__ MmaArgs p) {
@@ -292,13 +340,20 @@ __global__ void __launch_bounds__(kMmaThreads, 1) mma_kernel(const __grid_consta
   __shared__ MmaShared sh;
   uint8_t* ring = dyn + (1024 - smem_u32(dyn) % 1024) % 1024;
   const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
-  const int tile_bytes = p.tn * kMmaK, stage_bytes = kMmaRows * kMmaK + tile_bytes;
+  const int stage_bytes = kMmaRows * kMmaK + p.tn / (PAIR ? 2 : 1) * kMmaK;
   const int steps = (p.k + kMmaK - 1) / kMmaK;
-  const int rank = static_cast<int>(blockIdx.x) % p.split;
-  const int k0 = static_cast<int>(static_cast<int64_t>(steps) * rank / p.split);
-  const int k1 = static_cast<int>(static_cast<int64_t>(steps) * (rank + 1) / p.split);
+  // a cluster is a pair, the parts of k, or one block
+  const int cluster = PAIR ? 2 : p.split, rank = static_cast<int>(blockIdx.x) % cluster;
+  const int k0 = PAIR ? 0 : static_cast<int>(static_cast<int64_t>(steps) * rank / p.split);
+  const int k1 = PAIR ? steps : static_cast<int>(static_cast<int64_t>(steps) * (rank + 1) / p.split);
   const int64_t total = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
-  const int64_t t0 = blockIdx.x / p.split, dt = gridDim.x / p.split;
+  const int64_t t0 = blockIdx.x / cluster, dt = gridDim.x / cluster;
+  // rows of a in a tile, as many as the products' granularity makes of them
+  auto rows_of = [&](int im) {
+    const int left = static_cast<int>(min(static_cast<int64_t>(p.tn), p.m - static_cast<int64_t>(im) * p.tn));
+    return PAIR ? (left + 31) / 32 * 32 : (left + 15) / 16 * 16;
+  };
+  auto first_row_of = [&](int in) { return PAIR ? in * 2 * kMmaRows + rank * kMmaRows : in * kMmaRows; };
   int columns = 32;   // TMEM columns: two buffers, a power of two
   while (columns < 2 * p.tn) columns <<= 1;
 
@@ -310,7 +365,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) mma_kernel(const __grid_consta
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&sh.sum_full[i], 1);
-        mbar_init(&sh.sum_empty[i], 8);
+        mbar_init(&sh.sum_empty[i], (PAIR ? 2 : 1) * kEpiWarps);
       }
       mbar_init(&sh.drain, 1);
       sh.dead = 0;
@@ -318,13 +373,21 @@ __global__ void __launch_bounds__(kMmaThreads, 1) mma_kernel(const __grid_consta
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
   } else if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
-                 "r"(columns)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
+                   "r"(columns)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
+                   "r"(columns)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
     tmem_fence_before();
   }
   __syncthreads();
+  if (PAIR) cluster_sync();   // the other block's barriers are ready
   tmem_fence_after();
   const uint32_t tmem = sh.tmem;
 
@@ -342,9 +405,16 @@ __global__ void __launch_bounds__(kMmaThreads, 1) mma_kernel(const __grid_consta
             break;
           }
           uint8_t* dst = ring + s * stage_bytes;
-          mbar_expect(&sh.full[s], stage_bytes);
-          tma_load(dst, &map_b, kb * kMmaK, in * kMmaRows, &sh.full[s]);
-          tma_load(dst + kMmaRows * kMmaK, &map_a, kb * kMmaK, im * p.tn, &sh.full[s]);
+          if (PAIR) {
+            const uint32_t bar = in_block(&sh.full[s], 0);
+            if (rank == 0) mbar_expect(&sh.full[s], 2 * stage_bytes);
+            tma_load_pair(dst, &map_b, kb * kMmaK, first_row_of(in), bar);
+            tma_load_pair(dst + kMmaRows * kMmaK, &map_a, kb * kMmaK, im * p.tn + rank * (rows_of(im) / 2), bar);
+          } else {
+            mbar_expect(&sh.full[s], stage_bytes);
+            tma_load(dst, &map_b, kb * kMmaK, first_row_of(in), &sh.full[s]);
+            tma_load(dst + kMmaRows * kMmaK, &map_a, kb * kMmaK, im * p.tn, &sh.full[s]);
+          }
           issued = min(issued + 1, p.stages);
           if (++s == p.stages) {
             s = 0;
@@ -353,26 +423,24 @@ __global__ void __launch_bounds__(kMmaThreads, 1) mma_kernel(const __grid_consta
         }
       }
       // on giving up, copies may still be in flight: see each stage's last one
-      // through (a stage whose copy was consumed long ago has passed its phase)
-      if (!ok)
+      // through (a stage whose copy was consumed long ago has passed its phase);
+      // a pair's are counted by the first block, and the other ends after it
+      if (!ok && !(PAIR && rank))
         for (int i = 0; i < issued; ++i) {
           const int st = (s - 1 - i + 2 * p.stages) % p.stages;
           const uint32_t ph = st < s ? phase : phase ^ 1u;
-          const uint64_t w0 = now_ns();
-          while (!mbar_try(&sh.full[st], ph) && now_ns() - w0 < kWaitNs) {
-          }
+          mbar_drain(&sh.full[st], ph);
         }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && !(PAIR && rank)) {
       int s = 0, it = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int64_t t = t0; t < total && ok; t += dt, ++it) {
         int im, in;
         tile_at(p, t, im, in);
-        const int left = static_cast<int>(min(static_cast<int64_t>(p.tn), p.m - static_cast<int64_t>(im) * p.tn));
-        const uint32_t instr = i8_instr((left + 15) / 16 * 16);
+        const uint32_t instr = i8_instr<PAIR>(rows_of(im));
         const uint32_t d = tmem + static_cast<uint32_t>((it & 1) * p.tn);
         if (!mbar_wait(&sh.sum_empty[it & 1], ((it >> 1) & 1) ^ 1u, &sh.dead)) {
           ok = false;
@@ -389,37 +457,49 @@ __global__ void __launch_bounds__(kMmaThreads, 1) mma_kernel(const __grid_consta
           const uint64_t db = operand_desc(at), da = operand_desc(at + kMmaRows * kMmaK);
 #pragma unroll
           for (int q = 0; q < kMmaK / 32; ++q)   // 32 bytes of k an instruction
-            if (kb * kMmaK + q * 32 < p.k) mma_i8(d, db + 2 * q, da + 2 * q, instr, kb > k0 || q > 0);
-          mma_commit(&sh.empty[s]);
+            if (kb * kMmaK + q * 32 < p.k) mma_i8<PAIR>(d, db + 2 * q, da + 2 * q, instr, kb > k0 || q > 0);
+          mma_commit<PAIR>(&sh.empty[s]);
           if (++s == p.stages) {
             s = 0;
             phase ^= 1u;
           }
         }
-        if (ok) mma_commit(&sh.sum_full[it & 1]);
+        if (ok) mma_commit<PAIR>(&sh.sum_full[it & 1]);
       }
       if (!ok) {   // products that are still running
-        mma_commit(&sh.drain);
-        const uint64_t w0 = now_ns();
-        while (!mbar_try(&sh.drain, 0) && now_ns() - w0 < kWaitNs) {
-        }
+        mma_commit<PAIR>(&sh.drain);
+        mbar_drain(&sh.drain, 0);
       }
     }
-  } else if (p.split == 1) {
-    const int quarter = warp % 4, half = (warp - 2) / 4, etid = tid - 2 * kWarp;
-    const int cols = max(p.tn / 2, 16), c0 = half * cols;
+  } else if (PAIR || p.split == 1) {
+    const int quarter = warp % 4, etid = tid - 2 * kWarp;
+    const int cols = max(p.tn / (kEpiWarps / 4), 16), c0 = (warp - 2) / 4 * cols;
+    // scales of the next tile are fetched while this one is stored
+    float sa_next = 0.f, sb_next = 0.f, bias_next = 0.f;
+    auto fetch = [&](int64_t t) {
+      if (t >= total) return;
+      int im, in;
+      tile_at(p, t, im, in);
+      const int64_t mm = static_cast<int64_t>(im) * p.tn + etid;
+      const int64_t nn = static_cast<int64_t>(first_row_of(in)) + quarter * kWarp + lane;
+      sa_next = etid < p.tn && mm < p.m ? p.sa[mm] : 0.f;
+      sb_next = nn < p.n ? p.sb[nn] : 0.f;
+      bias_next = nn < p.n && p.bias ? p.bias[nn] : 0.f;
+    };
+    fetch(t0);
     int it = 0;
     for (int64_t t = t0; t < total; t += dt, ++it) {
       int im, in;
       tile_at(p, t, im, in);
       const int64_t m0 = static_cast<int64_t>(im) * p.tn;
-      const int64_t nn = static_cast<int64_t>(in) * kMmaRows + quarter * kWarp + lane;
+      const int64_t nn = static_cast<int64_t>(first_row_of(in)) + quarter * kWarp + lane;
       const int buf = it & 1;
-      if (etid < p.tn) sh.sa[buf][etid] = m0 + etid < p.m ? p.sa[m0 + etid] : 0.f;
+      if (etid < p.tn) sh.sa[buf][etid] = sa_next;
       const bool inside = nn < p.n, whole = __all_sync(kFull, inside);
-      float sb = inside ? p.sb[nn] : 0.f;
-      const float bias = inside && p.bias ? p.bias[nn] : 0.f;
+      float sb = sb_next;
+      const float bias = bias_next;
       epilogue_sync();
+      fetch(t + dt);
       // a block that gave up: NaN
       if (!__all_sync(kFull, mbar_wait(&sh.sum_full[buf], (it >> 1) & 1, &sh.dead))) sb = __int_as_float(0x7fc00000);
       tmem_fence_after();
@@ -460,13 +540,16 @@ __global__ void __launch_bounds__(kMmaThreads, 1) mma_kernel(const __grid_consta
       }
       tmem_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.sum_empty[buf]);
+      if (lane == 0) {
+        if (PAIR) mbar_arrive_at(in_block(&sh.sum_empty[buf], 0));
+        else mbar_arrive(&sh.sum_empty[buf]);
+      }
     }
   } else {
     mbar_wait(&sh.sum_full[0], 0, &sh.dead);
   }
 
-  if (p.split > 1) {
+  if (!PAIR && p.split > 1) {
     // one tile a cluster; this block has summed its part of k
     __syncwarp();
     tmem_fence_after();
@@ -476,20 +559,18 @@ __global__ void __launch_bounds__(kMmaThreads, 1) mma_kernel(const __grid_consta
     const int64_t m0 = static_cast<int64_t>(im) * p.tn;
     const int share = p.tn / p.split;   // columns of each block
     if (warp >= 2) {
-      const int quarter = warp % 4, half = (warp - 2) / 4;
-      const int cols = max(p.tn / 2, 16);
+      const int quarter = warp % 4, part = (warp - 2) / 4;
+      const int cols = max(p.tn / (kEpiWarps / 4), 16);
       const uint32_t at = tmem + (static_cast<uint32_t>(quarter * kWarp) << 16);
-      for (int c = half * cols; c < min(p.tn, (half + 1) * cols); c += 16) {
+      for (int c = part * cols; c < min(p.tn, (part + 1) * cols); c += 16) {
         int acc[16];
         tmem_load(at + c, acc);
         tmem_wait_load();
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int owner = (c + j) / share, slot = rank * share + (c + j) % share;
-          const uint32_t local = smem_u32(ring) + static_cast<uint32_t>((slot * kMmaRows + quarter * kWarp + lane) * 4);
-          uint32_t remote;
-          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(owner));
-          asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(remote), "r"(acc[j]) : "memory");
+          const int local = (slot * kMmaRows + quarter * kWarp + lane) * 4;
+          asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(in_block(ring + local, owner)), "r"(acc[j]) : "memory");
         }
       }
     }
@@ -497,9 +578,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1) mma_kernel(const __grid_consta
     cluster_sync();
     // a block that gave up has spoilt the sums of all of them
     for (int r = 0; r < p.split; ++r) {
-      uint32_t remote, v;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(&sh.dead)), "r"(r));
-      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
+      uint32_t v;
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(in_block(&sh.dead, r)) : "memory");
       bad |= v;
     }
     const int* recv = reinterpret_cast<const int*>(ring);
@@ -514,11 +594,16 @@ __global__ void __launch_bounds__(kMmaThreads, 1) mma_kernel(const __grid_consta
     }
     cluster_sync();   // the flags of this block are not read any more
   }
+  __syncwarp();
   tmem_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();   // neither block uses the other's memory any more
   if (warp == 1) {
     tmem_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+    if (PAIR)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
   }
 }
 
@@ -571,20 +656,22 @@ cudaError_t encode_rows(CUtensorMap* map, const int8_t* p, int64_t rows, int64_t
 
 struct MmaPlan {
   int tn, split;
+  bool pair;
 };
 
 // Rows of a in a tile: all of them up to 256, in steps that the two output
 // halves share; with more, 256, halved while the tiles do not fill the GPU.
 // A tile's k is split over 2, 4 or 8 blocks while blocks are idle and each
-// part keeps four steps of 128.
+// part keeps four steps of 128. Full-width tiles are made by pairs.
 MmaPlan plan_mma(int64_t m, int64_t n, int k, int sm_count) {
-  MmaPlan p{16, 1};
+  MmaPlan p{16, 1, false};
   while (p.tn < m && p.tn < kMmaMaxTn) p.tn <<= 1;
   const int64_t tn_tiles = (n + kMmaRows - 1) / kMmaRows;
   while (m > p.tn / 2 && p.tn > 64 && tn_tiles * ((m + p.tn - 1) / p.tn) * 2 <= sm_count) p.tn >>= 1;
   const int64_t tiles = tn_tiles * ((m + p.tn - 1) / p.tn);
   const int steps = (k + kMmaK - 1) / kMmaK;
   while (p.split < 8 && tiles * p.split * 2 <= sm_count && steps >= p.split * 8) p.split <<= 1;
+  p.pair = p.tn == kMmaMaxTn && p.split == 1 && n > kMmaRows;
   return p;
 }
 
@@ -607,27 +694,29 @@ cudaError_t launch_matmul_i8(const int8_t* a, int64_t m, int64_t as, const float
   p.tn = plan.tn;
   p.split = plan.split;
   p.pairs = os % 2 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0;
-  const int64_t tiles_m = (m + p.tn - 1) / p.tn, tiles_n = (n + kMmaRows - 1) / kMmaRows;
+  const int64_t rows = plan.pair ? 2 * kMmaRows : kMmaRows;
+  const int64_t tiles_m = (m + p.tn - 1) / p.tn, tiles_n = (n + rows - 1) / rows;
   p.tiles_m = static_cast<int>(tiles_m);
   p.tiles_n = static_cast<int>(tiles_n);
   // rows of a that stay in L2 beside the stream of b: about 32 MB
   p.group_m = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tiles_m, (32 << 20) / (static_cast<int64_t>(k) * p.tn + 1))));
-  const int stage = kMmaRows * kMmaK + p.tn * kMmaK;
+  const int a_rows = plan.pair ? p.tn / 2 : p.tn, cluster = plan.pair ? 2 : p.split;
+  const int stage = (kMmaRows + a_rows) * kMmaK;
   p.stages = std::min({kMmaMaxStages, (200 * 1024) / stage, std::max(2, (k + kMmaK - 1) / kMmaK * 2)});
   const size_t ring = std::max<size_t>(static_cast<size_t>(p.stages) * stage,
                                        p.split > 1 ? static_cast<size_t>(p.tn) * kMmaRows * 4 : 0);
   const size_t smem = ring + 1024;
   CUtensorMap ma, mb;
-  cudaError_t e = encode_rows(&ma, a, m, as, k, p.tn);
+  cudaError_t e = encode_rows(&ma, a, m, as, k, a_rows);
   if (e == cudaSuccess) e = encode_rows(&mb, b, n, bs, k, kMmaRows);
   if (e != cudaSuccess) return e;
-  const int64_t blocks = p.split > 1 ? tiles_m * tiles_n * p.split : std::min<int64_t>(tiles_m * tiles_n, sm_count);
+  const int64_t blocks = cluster * (p.split > 1 ? tiles_m * tiles_n : std::min<int64_t>(tiles_m * tiles_n, sm_count / cluster));
   auto run = [&](auto fn) -> cudaError_t {
     cudaError_t r = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (r != cudaSuccess) return r;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = static_cast<unsigned>(p.split);
+    attr.val.clusterDim.x = static_cast<unsigned>(cluster);
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(blocks));
@@ -638,9 +727,9 @@ cudaError_t launch_matmul_i8(const int8_t* a, int64_t m, int64_t as, const float
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, fn, ma, mb, p);
   };
-  if (dtype == GANN_F32) return run(mma_kernel<float>);
-  if (dtype == GANN_F16) return run(mma_kernel<__half>);
-  return run(mma_kernel<__nv_bfloat16>);
+  if (dtype == GANN_F32) return plan.pair ? run(mma_kernel<float, true>) : run(mma_kernel<float, false>);
+  if (dtype == GANN_F16) return plan.pair ? run(mma_kernel<__half, true>) : run(mma_kernel<__half, false>);
+  return plan.pair ? run(mma_kernel<__nv_bfloat16, true>) : run(mma_kernel<__nv_bfloat16, false>);
 }
 
 }  // namespace gann
