@@ -69,26 +69,129 @@ __device__ __forceinline__ int quant_code(float x, const RowScale& rs) {
   return rs.inv > 0.f ? static_cast<int>(fminf(fmaxf(r, -127.f), 127.f)) : 0;
 }
 
-// |x| for the maximum: a NaN becomes infinity, so it is not lost in fmaxf.
-__device__ __forceinline__ float mag(float x) { return isnan(x) ? INFINITY : fabsf(x); }
-
-// One warp per row.
 template <typename T>
-__global__ void __launch_bounds__(256) quantize_kernel(const uint8_t* __restrict__ x, int64_t rows, int64_t stride,
-                                                       int dim, int8_t* __restrict__ codes, int64_t cstride,
-                                                       float* __restrict__ scales) {
-  const int lane = threadIdx.x % kWarp;
-  const int64_t wpg = static_cast<int64_t>(gridDim.x) * (blockDim.x / kWarp);
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * (blockDim.x / kWarp) + threadIdx.x / kWarp; r < rows; r += wpg) {
+struct Row16 {   // 16 bytes of a row
+  static constexpr int n = 16 / sizeof(T);
+  uint4 v;
+  __device__ __forceinline__ float at(int j) const {
+    const uint32_t w = j * static_cast<int>(sizeof(T)) / 4 == 0   ? v.x
+                       : j * static_cast<int>(sizeof(T)) / 4 == 1 ? v.y
+                       : j * static_cast<int>(sizeof(T)) / 4 == 2 ? v.z
+                                                                  : v.w;
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w);
+    } else {
+      const uint16_t h = static_cast<uint16_t>((j & 1) ? w >> 16 : w);
+      return to_f32(*reinterpret_cast<const T*>(&h));
+    }
+  }
+};
+
+// Four codes of a word. With an ordinary scale the sum x / s + 1.5 * 2^23 holds
+// the rounded quotient in its low byte (|x / s| < 127.5); only an element whose
+// remainder is half a scale or more, where the product with the reciprocal may
+// have gone to the wrong side, takes the exact form above.
+__device__ __forceinline__ uint32_t quant_word(float x0, float x1, float x2, float x3, const RowScale& rs, bool plain) {
+  if (plain) {
+    constexpr float kMagic = 12582912.f;
+    const float a = __fadd_rn(__fmul_rn(x0, rs.inv), kMagic), b = __fadd_rn(__fmul_rn(x1, rs.inv), kMagic);
+    const float c = __fadd_rn(__fmul_rn(x2, rs.inv), kMagic), d = __fadd_rn(__fmul_rn(x3, rs.inv), kMagic);
+    const float ea = __fmaf_rn(kMagic - a, rs.s, x0), eb = __fmaf_rn(kMagic - b, rs.s, x1);
+    const float ec = __fmaf_rn(kMagic - c, rs.s, x2), ed = __fmaf_rn(kMagic - d, rs.s, x3);
+    const float e = fmaxf(fmaxf(fabsf(ea), fabsf(eb)), fmaxf(fabsf(ec), fabsf(ed)));
+    if (2.f * e < rs.s) {
+      const uint32_t lo = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040);
+      const uint32_t hi = __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040);
+      return __byte_perm(lo, hi, 0x5410);
+    }
+  }
+  return (quant_code(x0, rs) & 0xff) | (quant_code(x1, rs) & 0xff) << 8 | (quant_code(x2, rs) & 0xff) << 16 |
+         static_cast<uint32_t>(quant_code(x3, rs) & 0xff) << 24;
+}
+
+// A row by a group of threads: one warp, or (rows longer than a warp's
+// registers hold) a whole block. Bound by memory: 5 bytes move per float32
+// element, and the codes take about seven instructions each. The row's 16-byte
+// vectors (VEC: rows start on 16-byte boundaries) stay in registers between
+// the maximum and the codes, up to kRowHeld a thread; longer rows are read
+// again, which the caches serve.
+constexpr int kRowHeld = 8;
+
+template <typename T, bool VEC, int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * kWarp) quantize_kernel(
+    const uint8_t* __restrict__ x, int64_t rows, int64_t stride, int dim, int8_t* __restrict__ codes, int64_t cstride,
+    float* __restrict__ scales) {
+  constexpr int N = VEC ? Row16<T>::n : 1, NT = WARPS * kWarp;
+  __shared__ float red[WARPS];
+  const int t = WARPS == 1 ? threadIdx.x % kWarp : threadIdx.x;
+  const int per = WARPS == 1 ? 256 / kWarp : 1;   // rows of a block at a time
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * per + (WARPS == 1 ? threadIdx.x / kWarp : 0); r < rows;
+       r += static_cast<int64_t>(gridDim.x) * per) {
     const T* row = reinterpret_cast<const T*>(x + r * stride);
+    int8_t* out = codes + r * cstride;
+    const int nv = VEC ? dim / N : 0;   // whole vectors; the rest one by one
+    Row16<T> held[VEC ? kRowHeld : 1];
     float a = 0.f;
-    for (int j = lane; j < dim; j += kWarp) a = fmaxf(a, mag(to_f32(row[j])));
+    bool bad = false;
+    if constexpr (VEC) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) a = fmaxf(a, __shfl_xor_sync(kFull, a, o));
+      for (int i = 0; i < kRowHeld; ++i)
+        if (t + i * NT < nv) held[i].v = __ldcs(reinterpret_cast<const uint4*>(row) + t + i * NT);
+#pragma unroll
+      for (int i = 0; i < kRowHeld; ++i)
+        if (t + i * NT < nv) {
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            a = fmaxf(a, fabsf(held[i].at(j)));
+            bad |= isnan(held[i].at(j));
+          }
+        }
+      for (int v = t + kRowHeld * NT; v < nv; v += NT) {
+        Row16<T> w;
+        w.v = __ldg(reinterpret_cast<const uint4*>(row) + v);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          a = fmaxf(a, fabsf(w.at(j)));
+          bad |= isnan(w.at(j));
+        }
+      }
+    }
+    for (int j = nv * N + t; j < dim; j += NT) {
+      const float e = to_f32(row[j]);
+      a = fmaxf(a, fabsf(e));
+      bad |= isnan(e);
+    }
+    if (bad) a = INFINITY;
+    a = __uint_as_float(__reduce_max_sync(kFull, __float_as_uint(a)));   // not negative: bits are ordered
+    if constexpr (WARPS > 1) {
+      __syncthreads();
+      if (t % kWarp == 0) red[t / kWarp] = a;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) a = fmaxf(a, red[w]);
+    }
     const RowScale rs = row_scale(a);
-    for (int j = lane; j < dim; j += kWarp)
-      codes[r * cstride + j] = static_cast<int8_t>(quant_code(to_f32(row[j]), rs));
-    if (lane == 0) scales[r] = rs.scale;
+    const bool plain = rs.scale >= 0x1p-60f;   // not for tiny, zero and NaN scales
+    if constexpr (VEC) {
+      auto put = [&](const Row16<T>& w, int v) {
+        if constexpr (N == 4) {
+          reinterpret_cast<uint32_t*>(out)[v] = quant_word(w.at(0), w.at(1), w.at(2), w.at(3), rs, plain);
+        } else {
+          reinterpret_cast<uint2*>(out)[v] = make_uint2(quant_word(w.at(0), w.at(1), w.at(2), w.at(3), rs, plain),
+                                                        quant_word(w.at(4), w.at(5), w.at(6), w.at(7), rs, plain));
+        }
+      };
+#pragma unroll
+      for (int i = 0; i < kRowHeld; ++i)
+        if (t + i * NT < nv) put(held[i], t + i * NT);
+      for (int v = t + kRowHeld * NT; v < nv; v += NT) {
+        Row16<T> w;
+        w.v = __ldg(reinterpret_cast<const uint4*>(row) + v);
+        put(w, v);
+      }
+    }
+    for (int j = nv * N + t; j < dim; j += NT) out[j] = static_cast<int8_t>(quant_code(to_f32(row[j]), rs));
+    if (t == 0) scales[r] = rs.scale;
   }
 }
 
@@ -612,14 +715,27 @@ __global__ void __launch_bounds__(kMmaThreads, 1) mma_kernel(const __grid_consta
 cudaError_t launch_quantize_rows(const void* x, int64_t rows, int64_t stride, int dim, int dtype, int8_t* codes,
                                  int64_t code_stride, float* scales, int sm_count, cudaStream_t st) {
   if (rows <= 0) return cudaSuccess;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((rows + 7) / 8, static_cast<int64_t>(sm_count) * 32));
-  auto run = [&](auto fn) {
-    fn<<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(x), rows, stride, dim, codes, code_stride, scales);
+  const bool vec = stride % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  // one warp a row while its registers hold it, or there are rows enough to
+  // fill the GPU with single warps
+  const int held = kRowHeld * kWarp * (dtype == GANN_F32 ? 4 : 8);
+  const bool block = dim > held && rows < static_cast<int64_t>(sm_count) * 64;
+  auto run = [&](auto one, auto many) {
+    const int64_t grid = block ? std::min<int64_t>(rows, static_cast<int64_t>(sm_count) * 16)
+                               : std::min<int64_t>((rows + 7) / 8, static_cast<int64_t>(sm_count) * 32);
+    auto fn = block ? many : one;
+    fn<<<static_cast<unsigned>(grid), block ? 512 : 256, 0, st>>>(static_cast<const uint8_t*>(x), rows, stride, dim,
+                                                                  codes, code_stride, scales);
     return cudaGetLastError();
   };
-  if (dtype == GANN_F32) return run(quantize_kernel<float>);
-  if (dtype == GANN_F16) return run(quantize_kernel<__half>);
-  return run(quantize_kernel<__nv_bfloat16>);
+  if (dtype == GANN_F32)
+    return vec ? run(quantize_kernel<float, true, 1>, quantize_kernel<float, true, 16>)
+               : run(quantize_kernel<float, false, 1>, quantize_kernel<float, false, 16>);
+  if (dtype == GANN_F16)
+    return vec ? run(quantize_kernel<__half, true, 1>, quantize_kernel<__half, true, 16>)
+               : run(quantize_kernel<__half, false, 1>, quantize_kernel<__half, false, 16>);
+  return vec ? run(quantize_kernel<__nv_bfloat16, true, 1>, quantize_kernel<__nv_bfloat16, true, 16>)
+             : run(quantize_kernel<__nv_bfloat16, false, 1>, quantize_kernel<__nv_bfloat16, false, 16>);
 }
 
 namespace {

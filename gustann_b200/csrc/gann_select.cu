@@ -947,30 +947,60 @@ struct StateTable {
   gann_state s[kStateBatch];
 };
 
-// One CTA per (state, group, slice of the row's bytes): a thread owns one unit
-// of the row in every beam, reads all of them that a kept row needs and then
-// writes them, so source and target may be the same rows.
-template <typename U>
+// A thread owns one unit of U bytes at one place of a group's blocks, in every
+// beam. MAX > 0: it reads the unit of every kept row (at most MAX) before it
+// writes any, so source and target may be the same rows; rows that stay where
+// they are are not touched. MAX 0: source and target are apart, and eight rows
+// at a time are on their way. Bound by memory: each kept row is written once
+// and each distinct parent read once from DRAM (again from the caches).
+template <typename U, int MAX>
 __global__ void __launch_bounds__(256) reorder_kernel(const __grid_constant__ StateTable tab,
                                                       const int32_t* __restrict__ parents, int beams, int keep) {
   const gann_state& s = tab.s[blockIdx.z];
   const int64_t g = blockIdx.y;
-  const int32_t* par = parents + g * keep;
+  __shared__ int32_t par[kBeamMax];
+  for (int j = threadIdx.x; j < keep; j += blockDim.x) {
+    const int b = parents[g * keep + j];
+    par[j] = b >= 0 && b < beams ? b : -1;
+  }
+  __syncthreads();
   const int64_t units = s.row_bytes / static_cast<int64_t>(sizeof(U));
   const int64_t total = s.size[0] * s.size[1] * units;
   const uint8_t* src = static_cast<const uint8_t*>(s.src) + g * s.src_group;
   uint8_t* dst = static_cast<uint8_t*>(s.dst) + g * s.dst_group;
+  const bool same = s.src == s.dst;
   for (int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; e < total;
        e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t u = e % units, r = e / units, i1 = r % s.size[1], i0 = r / s.size[1];
+    int64_t u, i0, i1;
+    if (total < (int64_t(1) << 31)) {
+      const uint32_t r = static_cast<uint32_t>(e) / static_cast<uint32_t>(units);
+      u = static_cast<uint32_t>(e) - r * static_cast<uint32_t>(units);
+      i0 = r / static_cast<uint32_t>(s.size[1]);
+      i1 = r - static_cast<uint32_t>(i0) * static_cast<uint32_t>(s.size[1]);
+    } else {
+      const int64_t r = e / units;
+      u = e - r * units;
+      i0 = r / s.size[1];
+      i1 = r - i0 * s.size[1];
+    }
     const uint8_t* p = src + i0 * s.src_stride[0] + i1 * s.src_stride[1] + u * static_cast<int64_t>(sizeof(U));
     uint8_t* q = dst + i0 * s.dst_stride[0] + i1 * s.dst_stride[1] + u * static_cast<int64_t>(sizeof(U));
-    U v[kBeamMax];
-    for (int j = 0; j < keep; ++j) {
-      const int b = par[j];
-      v[j] = b >= 0 && b < beams ? *reinterpret_cast<const U*>(p + b * s.src_beam) : U{};
+    constexpr int V = MAX ? MAX : 8;
+    for (int j0 = 0; j0 < (MAX ? 1 : keep); j0 += V) {
+      U v[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        v[j] = U{};
+        if (j0 + j < keep) {
+          const int b = par[j0 + j];
+          if (b >= 0 && !(MAX && same && b == j)) v[j] = *reinterpret_cast<const U*>(p + b * s.src_beam);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j0 + j < keep && !(MAX && same && par[j0 + j] == j))
+          *reinterpret_cast<U*>(q + (j0 + j) * s.dst_beam) = v[j];
     }
-    for (int j = 0; j < keep; ++j) *reinterpret_cast<U*>(q + j * s.dst_beam) = v[j];
   }
 }
 
@@ -1092,30 +1122,67 @@ cudaError_t launch_beam_select(const SelectArgs& a, int sm_count, cudaStream_t s
   return run_select<__nv_bfloat16>(a, sm_count, st);
 }
 
+namespace {
+
+// The widest unit that all addresses, strides and rows of the states allow.
+int state_unit(const gann_state* s, int count) {
+  int64_t bits = 16;
+  for (int i = 0; i < count; ++i)
+    bits |= static_cast<int64_t>(reinterpret_cast<uintptr_t>(s[i].src)) | static_cast<int64_t>(reinterpret_cast<uintptr_t>(s[i].dst)) |
+            s[i].src_group | s[i].src_beam | s[i].dst_group | s[i].dst_beam | s[i].row_bytes | s[i].src_stride[0] |
+            s[i].src_stride[1] | s[i].dst_stride[0] | s[i].dst_stride[1];
+  return static_cast<int>(bits & -bits);
+}
+
+template <typename U>
+cudaError_t run_reorder(const StateTable& t, bool in_place, const dim3& grid, const int32_t* parents, int beams,
+                        int keep, cudaStream_t st) {
+  if (!in_place) reorder_kernel<U, 0><<<grid, 256, 0, st>>>(t, parents, beams, keep);
+  else if (keep <= 8) reorder_kernel<U, 8><<<grid, 256, 0, st>>>(t, parents, beams, keep);
+  else if (keep <= 32) reorder_kernel<U, 32><<<grid, 256, 0, st>>>(t, parents, beams, keep);
+  else if constexpr (sizeof(U) <= 4) reorder_kernel<U, kBeamMax><<<grid, 256, 0, st>>>(t, parents, beams, keep);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
 cudaError_t launch_reorder_states(const gann_state* states, int count, const int32_t* parents, int64_t groups,
                                   int beams, int keep, int sm_count, cudaStream_t st) {
-  (void)sm_count;
-  for (int lo = 0; lo < count; lo += kStateBatch) {
-    const int c = std::min(kStateBatch, count - lo);
-    StateTable tab{};
-    int64_t most = 0;
-    for (int i = 0; i < c; ++i) {
-      tab.s[i] = states[lo + i];
-      most = std::max(most, tab.s[i].size[0] * tab.s[i].size[1] * tab.s[i].row_bytes);
-    }
-    if (most == 0) continue;
-    for (int64_t g0 = 0; g0 < groups; g0 += 65535) {
-      const int64_t gn = std::min<int64_t>(65535, groups - g0);
-      StateTable t = tab;
-      for (int i = 0; i < c; ++i) {
-        t.s[i].src = static_cast<const uint8_t*>(tab.s[i].src) + g0 * tab.s[i].src_group;
-        t.s[i].dst = static_cast<uint8_t*>(tab.s[i].dst) + g0 * tab.s[i].dst_group;
+  // states of the same kind (in place or not) and alignment share launches
+  for (int kind = 0; kind < 10; ++kind) {
+    const bool in_place = kind >= 5;
+    const int unit = 1 << (kind % 5);
+    for (int next = 0; next < count;) {
+      StateTable tab{};
+      int c = 0;
+      int64_t most = 0;
+      for (; next < count && c < kStateBatch; ++next) {
+        const gann_state& s = states[next];
+        const int64_t size = s.size[0] * s.size[1] * s.row_bytes;
+        if (size == 0 || (s.src == s.dst) != in_place || state_unit(&s, 1) != unit) continue;
+        tab.s[c++] = s;
+        most = std::max(most, size);
       }
-      const dim3 grid(static_cast<unsigned>(std::min<int64_t>((most + 255) / 256, 1024)), static_cast<unsigned>(gn),
-                      static_cast<unsigned>(c));
-      reorder_kernel<uint8_t><<<grid, 256, 0, st>>>(t, parents + g0 * keep, beams, keep);
-      const cudaError_t e = cudaGetLastError();
-      if (e != cudaSuccess) return e;
+      if (c == 0) break;
+      // 128 rows at a time in registers: at most 4 bytes of each
+      const int width = in_place && keep > 32 ? std::min(unit, 4) : unit;
+      const int64_t blocks = std::min<int64_t>((most / width + 255) / 256, static_cast<int64_t>(sm_count) * 1024);
+      for (int64_t g0 = 0; g0 < groups; g0 += 65535) {
+        StateTable t = tab;
+        for (int i = 0; i < c; ++i) {
+          t.s[i].src = static_cast<const uint8_t*>(tab.s[i].src) + g0 * tab.s[i].src_group;
+          t.s[i].dst = static_cast<uint8_t*>(tab.s[i].dst) + g0 * tab.s[i].dst_group;
+        }
+        const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(std::min<int64_t>(65535, groups - g0)),
+                        static_cast<unsigned>(c));
+        const int32_t* par = parents + g0 * keep;
+        const cudaError_t e = width == 16  ? run_reorder<uint4>(t, in_place, grid, par, beams, keep, st)
+                              : width == 8 ? run_reorder<uint2>(t, in_place, grid, par, beams, keep, st)
+                              : width == 4 ? run_reorder<uint32_t>(t, in_place, grid, par, beams, keep, st)
+                              : width == 2 ? run_reorder<uint16_t>(t, in_place, grid, par, beams, keep, st)
+                                           : run_reorder<uint8_t>(t, in_place, grid, par, beams, keep, st);
+        if (e != cudaSuccess) return e;
+      }
     }
   }
   return cudaSuccess;
