@@ -155,17 +155,6 @@ __device__ __forceinline__ void warp_sort(K (&k)[N], int lane) {
   }
 }
 
-// The r-th largest (r <= 32) of the warp's 32 values as ord32 keys (0: none).
-__device__ __forceinline__ uint32_t warp_rth(uint32_t u, int r, int lane) {
-  uint32_t w = __reduce_max_sync(kFull, u);
-  for (int i = 1; i < r; ++i) {
-    const unsigned m = __ballot_sync(kFull, u == w);
-    if (lane == __ffs(m) - 1) u = 0;
-    w = __reduce_max_sync(kFull, u);
-  }
-  return w;
-}
-
 // The warp's 32 values sorted, largest first.
 __device__ __forceinline__ float warp_sort32(float v, int lane) {
 #pragma unroll
@@ -184,21 +173,6 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 constexpr float kLog2e = 1.4426950408889634f;
-
-// Sum of one int a thread over the block; `red` holds a word for each warp.
-// The barriers around it make it safe to call in a loop.
-template <int NW>
-__device__ __forceinline__ int block_sum(int c, int* red) {
-  c = __reduce_add_sync(kFull, c);
-  if (NW == 1) return c;
-  if (threadIdx.x % kWarp == 0) red[threadIdx.x / kWarp] = c;
-  __syncthreads();
-  int s = 0;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) s += red[w];
-  __syncthreads();
-  return s;
-}
 
 __device__ __forceinline__ bool live(float score) { return fabsf(score) < INFINITY; }
 
@@ -300,7 +274,7 @@ __global__ void __launch_bounds__(kRowWarps* kWarp, 5) row_kernel(const T* __res
   Key1* list = lists[warp];
   Key1 floor{0};   // the least kept key once `keep` are known
   int cnt = 0;
-  float thr = -INFINITY, m = -INFINITY;
+  float thr = -INFINITY, m = -INFINITY, m2 = 0.f, fix = 1.f;
   auto cut = [&]() {
     sort_some<LONG>(list, cnt, keep, lane, [&](int i) { return list[i]; });
     cnt = min(cnt, keep);
@@ -357,9 +331,11 @@ __global__ void __launch_bounds__(kRowWarps* kWarp, 5) row_kernel(const T* __res
       uint32_t mark = 0;
 #pragma unroll
       for (int i = 0; i < kRowVecs; ++i)
+        if (vm[i] >= thr) {
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-          if (Raw<T>::at(cur[i], j) >= thr) mark |= 1u << (i * N + j);
+          for (int j = 0; j < N; ++j)
+            if (Raw<T>::at(cur[i], j) >= thr) mark |= 1u << (i * N + j);
+        }
       while (__any_sync(kFull, mark)) {
         if (cnt > kCap - kWarp) cut();
         const int e = __ffs(mark) - 1;
@@ -372,19 +348,26 @@ __global__ void __launch_bounds__(kRowWarps* kWarp, 5) row_kernel(const T* __res
         cnt += __popc(pass);
         mark &= mark - 1;
       }
+      // a higher threshold is worth a short sort
+      if (cnt > max(16, 2 * keep)) cut();
     }
     if (SOFTMAX) {
       if (mx > m) {
         sum *= static_cast<double>(fast_exp2((m - mx) * kLog2e));
         m = mx;
+        m2 = m * kLog2e;
+        fix = 1.f - __fmaf_rn(m, kLog2e, -m2) * 0.6931471805599453f;
       }
       float part = 0.f;
       if (m > -INFINITY) {
+        // 2^(x log2e - m2), one fused step an element; `fix` makes up for m2's
+        // rounding
 #pragma unroll
         for (int i = 0; i < kRowVecs; ++i)
 #pragma unroll
-          for (int j = 0; j < N; ++j) part += fast_exp2((Raw<T>::at(cur[i], j) - m) * kLog2e);
-        if (!(part < INFINITY)) {   // a NaN or an infinite entry: again without them
+          for (int j = 0; j < N; ++j) part += fast_exp2(__fmaf_rn(Raw<T>::at(cur[i], j), kLog2e, -m2));
+        part *= fix;
+        if (!(part >= 0.f && part < INFINITY)) {   // a NaN or infinite entry, or m2 past float32: again without
           part = 0.f;
 #pragma unroll
           for (int i = 0; i < kRowVecs; ++i)
@@ -413,20 +396,21 @@ __global__ void __launch_bounds__(kRowWarps* kWarp, 5) row_kernel(const T* __res
 }
 
 // ------------------------------------------------------------ whole groups
-// Many groups, no softmax: a warp takes a whole group, in tiles of 16 to
-// 64 elements a lane in registers, vectors of 16 bytes (single elements when rows
-// are not whole vectors). f = fl32(x + S_b) orders candidates as their 64-bit
-// values do, up to equality. The first tile sets a threshold of f: the keep-th
-// largest of the lanes' maxima (keep <= 16), or one bisected until between
-// `keep` and 128 elements pass. Lanes mark the elements with x >= thr - S_b (a
-// little less, so none with f >= thr is missed); the marked ones are valued
-// in 64 bits, compared with the least kept key and listed.
+// Many groups, no softmax: a warp takes a whole group, in tiles of NV vectors a
+// lane (16 bytes, or single elements when rows are not whole vectors), of which
+// only the maxima stay in registers. f = fl32(x + S_b) orders candidates as
+// their 64-bit values do, up to equality. The first tile sets a threshold of
+// f: the keep-th largest of the lanes' maxima (keep <= 16), or of the vectors'
+// by bisection, has `keep` elements at or above it. Vectors whose maximum
+// passes are read again (from L1), one a lane at a time, and their elements at
+// or above the threshold are listed as (f, index); the sort by that is looked
+// over for equal f, which are put in the order of their 64-bit values.
 constexpr int kGroupWarps = 4;
 
 template <typename T, int VW>
 struct Vec {
   uint4 v;
-  __device__ __forceinline__ void load(const T* p) { v = __ldcs(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void load(const T* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
   __device__ __forceinline__ float at(int j) const { return Raw<T>::at(v, j); }
   __device__ __forceinline__ float max() const { return Raw<T>::max(v); }
 };
@@ -438,14 +422,13 @@ struct Vec<T, 1> {
   __device__ __forceinline__ float max() const { return v; }
 };
 
-template <typename T, int VW, int ELEMS, bool LONG>
-__global__ void __launch_bounds__(kGroupWarps* kWarp, LONG || ELEMS > 32 ? 4 : 6) group_kernel(
+template <typename T, int VW, int NV, bool LONG>
+__global__ void __launch_bounds__(kGroupWarps* kWarp, NV * VW > 32 ? 5 : 7) group_kernel(
     const T* __restrict__ logits, int64_t gstride, int64_t bstride, const float* __restrict__ scores,
     const uint8_t* __restrict__ finished, int64_t groups, int beams, int vocab, int keep, int end_token, uint32_t magic,
     int shift, float* __restrict__ out_s, int32_t* __restrict__ out_p, int32_t* __restrict__ out_t) {
-  constexpr int NV = ELEMS / VW, kCap = Held<LONG>::value;
-  using Mark = typename std::conditional<(ELEMS > 32), unsigned long long, uint32_t>::type;
-  __shared__ Key2 lists[kGroupWarps][kCap];
+  constexpr int kCap = Held<LONG>::value;
+  __shared__ Key1 lists[kGroupWarps][kCap];
   __shared__ float cs[kGroupWarps][kBeamMax];
   const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
   const int64_t g = static_cast<int64_t>(blockIdx.x) * kGroupWarps + warp;
@@ -453,23 +436,33 @@ __global__ void __launch_bounds__(kGroupWarps* kWarp, LONG || ELEMS > 32 ? 4 : 6
   const T* base = logits + g * gstride;
   const float* sc = scores + g * beams;
   float* c = cs[warp];
-  Key2* list = lists[warp];
+  Key1* list = lists[warp];
   const uint32_t vr = static_cast<uint32_t>(vocab) / VW, nvec = vr * beams;
-  const bool joined = bstride == vocab;
   // row of a vector: division by the row's length as a product (magic =
   // ceil(2^(32+shift) / vr), exact below 2^31)
   auto row_of = [&](uint32_t v) { return (magic ? __umulhi(v, magic) : v) >> shift; };
-  Vec<T, VW> raw[NV];
+  auto where = [&](uint32_t v) {
+    const uint32_t b = row_of(v);
+    return base + b * bstride + static_cast<int64_t>(v - b * vr) * VW;
+  };
+  const bool joined = bstride == vocab;
+  float f[NV];   // of the vectors' maxima; NaN: nothing there
   auto load = [&](uint32_t t0) {
+    Vec<T, VW> raw[NV];
+    if (joined && t0 + NV * kWarp <= nvec) {
+      const T* p = base + static_cast<int64_t>(t0 + lane) * VW;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const uint32_t v = t0 + i * kWarp + lane;
-      if (v < nvec) {
-        if (joined) {
-          raw[i].load(base + static_cast<int64_t>(v) * VW);
-        } else {
-          const uint32_t b = row_of(v);
-          raw[i].load(base + b * bstride + static_cast<int64_t>(v - b * vr) * VW);
+      for (int i = 0; i < NV; ++i) raw[i].load(p + i * kWarp * VW);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) f[i] = raw[i].max();
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const uint32_t v = t0 + i * kWarp + lane;
+        f[i] = kNan;
+        if (v < nvec) {
+          raw[i].load(where(v));
+          f[i] = raw[i].max();
         }
       }
     }
@@ -480,67 +473,94 @@ __global__ void __launch_bounds__(kGroupWarps* kWarp, LONG || ELEMS > 32 ? 4 : 6
     c[b] = live(s) && !(finished && finished[g * beams + b]) ? s : kNan;
   }
   __syncwarp();
+
   int cnt = 0;
-  Key2 floor{0, 0};   // the least kept key once `keep` are known
-  float thr = -INFINITY;
-  auto cut = [&]() {
-    sort_some<LONG>(list, cnt, keep, lane, [&](int i) { return list[i]; });
-    cnt = min(cnt, keep);
-    if (cnt < keep) return;
-    floor = list[keep - 1];
-    thr = static_cast<float>(unord64(floor.a));
+  bool full = false;       // `keep` candidates are known: the last one is the floor
+  float thr = -INFINITY;   // candidates have f >= thr
+  double floor_v = 0.0;
+  uint32_t floor_id = 0;
+  auto value = [&](uint32_t id) {
+    const uint32_t b = row_of(id / VW);
+    if (isnan(c[b])) return static_cast<double>(sc[b]);   // a finished beam's candidate
+    return static_cast<double>(c[b]) + static_cast<double>(Raw<T>::one(base + b * bstride + (id - b * vocab)));
   };
+  auto cut = [&]() {
+    const int total = cnt;
+    sort_some<LONG>(list, total, total, lane, [&](int i) { return list[i]; });
+    bool equal = false;
+    for (int i = lane; i + 1 < total && i < keep; i += kWarp) equal |= (list[i].a >> 32) == (list[i + 1].a >> 32);
+    if (__any_sync(kFull, equal)) {
+      for (bool moved = true; moved;) {
+        moved = false;
+        for (int odd = 0; odd < 2; ++odd) {
+          for (int i = odd + 2 * lane; i + 1 < total; i += 2 * kWarp) {
+            const Key1 x = list[i], y = list[i + 1];
+            if ((x.a >> 32) == (y.a >> 32) && value(~static_cast<uint32_t>(x.a)) < value(~static_cast<uint32_t>(y.a))) {
+              list[i] = y;
+              list[i + 1] = x;
+              moved = true;
+            }
+          }
+          __syncwarp();
+        }
+        moved = __any_sync(kFull, moved);
+      }
+    }
+    cnt = min(total, keep);
+    full = cnt == keep;
+    if (!full) return;
+    floor_id = ~static_cast<uint32_t>(list[keep - 1].a);
+    floor_v = value(floor_id);
+    thr = unord32(static_cast<uint32_t>(list[keep - 1].a >> 32));
+  };
+
   for (uint32_t t0 = 0; t0 < nvec; t0 += NV * kWarp) {
     if (t0) load(t0);
-    float cb[NV];   // NaN: a row without elements, or nothing there
+    float mx = -INFINITY;
+    bool inf = false;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      inf |= f[i] == INFINITY;
       const uint32_t v = t0 + i * kWarp + lane;
-      cb[i] = v < nvec ? c[row_of(v)] : kNan;
+      f[i] = __fadd_rn(f[i], c[row_of(min(v, nvec - 1))]);
+      mx = fmaxf(mx, f[i]);
+    }
+    if (__any_sync(kFull, inf)) {   // masked entries: maxima without them
+      mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const uint32_t v = t0 + i * kWarp + lane;
+        f[i] = kNan;
+        if (v < nvec) {
+          Vec<T, VW> w;
+          w.load(where(v));
+          float x = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < VW; ++j)
+            if (w.at(j) < INFINITY) x = fmaxf(x, w.at(j));
+          f[i] = __fadd_rn(x, c[row_of(v)]);
+          mx = fmaxf(mx, f[i]);
+        }
+      }
     }
     if (t0 == 0) {
       if (!LONG) {
-        // rounding keeps order, so one sum a vector; masked entries that are
-        // +infinity have to be left out
-        float mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) mx = fmaxf(mx, __fadd_rn(raw[i].max(), cb[i]));
-        if (mx == INFINITY) {
-          mx = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < VW; ++j)
-              if (raw[i].at(j) < INFINITY) mx = fmaxf(mx, __fadd_rn(raw[i].at(j), cb[i]));
-        }
         thr = __shfl_sync(kFull, warp_sort32(mx, lane), keep - 1);
       } else {
         // bisection by value, then (far from done) over the order of floats
-        float hi = -INFINITY, lo = -INFINITY, low = INFINITY;
+        float lo = -INFINITY, low = INFINITY;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-#pragma unroll
-          for (int j = 0; j < VW; ++j) {
-            const float x = raw[i].at(j), f = __fadd_rn(x, cb[i]);
-            if (fabsf(x) < INFINITY && fabsf(f) < INFINITY) {
-              hi = fmaxf(hi, f);
-              low = fminf(low, f);
-            }
-          }
-        hi = unord32(__reduce_max_sync(kFull, ord32(hi)));
+          if (f[i] > -INFINITY) low = fminf(low, f[i]);
+        float hi = unord32(__reduce_max_sync(kFull, ord32(mx)));
         float mid = -unord32(__reduce_max_sync(kFull, ord32(-low)));
         for (int r = 0; r < 24 && hi > mid; ++r) {
           int n = 0;
 #pragma unroll
-          for (int i = 0; i < NV; ++i)
-            if (i * kWarp < nvec) {
-#pragma unroll
-              for (int j = 0; j < VW; ++j) n += __fadd_rn(raw[i].at(j), cb[i]) >= mid && raw[i].at(j) < INFINITY;
-            }
-          n = __reduce_add_sync(kFull, n);
+          for (int i = 0; i < NV; ++i) n += __popc(__ballot_sync(kFull, f[i] >= mid));
           if (n >= keep) {
             lo = mid;
-            if (n <= 128) break;
+            if (n <= keep + 4) break;
           } else {
             hi = mid;
           }
@@ -552,393 +572,196 @@ __global__ void __launch_bounds__(kGroupWarps* kWarp, LONG || ELEMS > 32 ? 4 : 6
         thr = lo;
       }
     }
-    Mark mark = 0;
-    const float below = thr - fabsf(thr) * 0x1p-23f;   // by half a step of thr at least
+    uint32_t vecs = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const float least = __fadd_rd(below, -cb[i]);
-#pragma unroll
-      for (int j = 0; j < VW; ++j)
-        if (raw[i].at(j) >= least) mark |= Mark(1) << (i * VW + j);
-    }
-    int b0 = 0;
+    for (int i = 0; i < NV; ++i)
+      if (f[i] >= thr) vecs |= 1u << i;
+    // one element a lane a round; finished beams, one candidate each, behind
+    // the first tile's
+    Vec<T, VW> w;
+    uint32_t elems = 0, id0 = 0;
+    float cb = kNan;
+    int b0 = finished && t0 == 0 ? 0 : beams;
     while (true) {
-      bool take = mark != 0;
-      double v = 0.0;
+      bool take = false;
+      float fx = kNan;
       uint32_t id = 0;
-      if (__any_sync(kFull, take)) {
-        if (take) {
-          const int e = (ELEMS > 32 ? __ffsll(mark) : __ffs(static_cast<uint32_t>(mark))) - 1;
-          id = (t0 + (e / VW) * kWarp + lane) * VW + e % VW;
-          const uint32_t b = row_of(id / VW);
-          const float x = Raw<T>::one(base + b * bstride + (id - b * vocab));
-          take = fabsf(x) < INFINITY;
-          v = static_cast<double>(c[b]) + static_cast<double>(x);
-          mark &= mark - 1;
+      if (__any_sync(kFull, vecs | elems)) {
+        if (!elems && vecs) {
+          const uint32_t v = t0 + (__ffs(vecs) - 1) * kWarp + lane;
+          vecs &= vecs - 1;
+          w.load(where(v));
+          cb = c[row_of(v)];
+          id0 = v * VW;
+#pragma unroll
+          for (int j = 0; j < VW; ++j)
+            if (__fadd_rn(w.at(j), cb) >= thr && fabsf(w.at(j)) < INFINITY) elems |= 1u << j;
         }
-      } else {
-        if (!finished || t0 || b0 >= beams) break;
+        if (elems) {
+          const int e = __ffs(elems) - 1;
+          elems &= elems - 1;
+          float x = w.at(0);
+#pragma unroll
+          for (int j = 1; j < VW; ++j)
+            if (e == j) x = w.at(j);
+          fx = __fadd_rn(x, cb);
+          id = id0 + e;
+          take = true;
+        }
+      } else if (b0 < beams) {
         const int b = b0 + lane;
         take = b < beams && isnan(c[b]) && live(sc[b]);
         if (take) {
-          v = static_cast<double>(sc[b]);
+          fx = sc[b];
           id = static_cast<uint32_t>(b) * vocab + end_token;
         }
         b0 += kWarp;
+      } else {
+        break;
       }
       if (cnt > kCap - kWarp) cut();
-      const Key2 k{ord64(v), ~id};
+      take = take && fx >= thr;
+      if (full && take && fx == thr) {
+        const double v = value(id);
+        take = v > floor_v || (v == floor_v && id < floor_id);
+      }
+      const unsigned pass = __ballot_sync(kFull, take);
+      if (take) list[cnt + __popc(pass & ((1u << lane) - 1u))] = {(static_cast<uint64_t>(ord32(fx)) << 32) | ~id};
+      cnt += __popc(pass);
+    }
+    if (t0 + NV * kWarp >= nvec || cnt > (LONG ? kCap / 2 : max(16, 2 * keep))) cut();
+  }
+  __syncwarp();
+  for (int j = lane; j < keep; j += kWarp) {
+    const bool ok = j < cnt;
+    const uint32_t idx = ok ? ~static_cast<uint32_t>(list[j].a) : 0u, b = row_of(idx / VW);
+    out_s[g * keep + j] = ok ? static_cast<float>(value(idx)) : -INFINITY;
+    out_p[g * keep + j] = ok ? static_cast<int32_t>(b) : -1;
+    out_t[g * keep + j] = ok ? static_cast<int32_t>(idx - b * vocab) : -1;
+  }
+}
+
+// ------------------------------------------------------------------- join
+// The segments' candidates of one group: a block a group. Warps join rows'
+// sums, then each takes a part of the candidates, values them in 64 bits and
+// keeps its best in a sorted list; a candidate's place in the result is its
+// place in its own list plus, for every other list, the number of keys above
+// it (binary search).
+constexpr int kMergeWarps = 8;
+
+template <bool LONG>
+__global__ void __launch_bounds__(kMergeWarps* kWarp) merge_kernel(
+    const Key1* __restrict__ cand, const SegStat* __restrict__ stats, const float* __restrict__ scores,
+    const uint8_t* __restrict__ finished, int64_t groups, int beams, int vocab, int keep, int segs, int softmax,
+    int end_token, float* __restrict__ out_s, int32_t* __restrict__ out_p, int32_t* __restrict__ out_t) {
+  constexpr int kCap = Held<LONG>::value;
+  __shared__ double offs[kBeamMax], tops[kBeamMax];   // v = offs + (x - tops)
+  __shared__ uint8_t kind[kBeamMax];                  // 0 no candidates, 1 lists, 2 finished
+  __shared__ Key2 lists[kMergeWarps][kCap];
+  __shared__ int counts[kMergeWarps];
+  const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
+  cudaGridDependencySynchronize();
+  const int64_t per_beam = static_cast<int64_t>(segs) * keep, total = per_beam * beams;
+  const bool small = total < (int64_t(1) << 31);
+  for (int64_t g = blockIdx.x; g < groups; g += gridDim.x) {
+    const float* sc = scores + g * beams;
+    for (int b = warp; b < beams; b += kMergeWarps) {
+      const float s = sc[b];
+      const bool fin = finished && finished[g * beams + b];
+      double mx = -INFINITY, sum = 0.0;
+      if (softmax && !fin && live(s)) {
+        const SegStat* st = stats + (g * beams + b) * segs;
+        for (int i = lane; i < segs; i += kWarp) mx = fmax(mx, st[i].max);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) mx = fmax(mx, __shfl_xor_sync(kFull, mx, o));
+        if (mx > -INFINITY)
+          for (int i = lane; i < segs; i += kWarp)
+            if (st[i].sum > 0.0) sum += st[i].sum * exp(st[i].max - mx);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+      }
+      if (lane == 0) {
+        kind[b] = !live(s) ? 0 : fin ? 2 : 1;
+        offs[b] = static_cast<double>(s) - (sum > 0.0 ? log(sum) : 0.0);
+        tops[b] = mx > -INFINITY ? mx : 0.0;
+      }
+    }
+    __syncthreads();
+    // at least 32 candidates a warp, and no more warps than that needs
+    const int warps = static_cast<int>(min(static_cast<int64_t>(kMergeWarps), (total + kWarp - 1) / kWarp));
+    const int64_t e0 = total * warp / warps, e1 = warp < warps ? total * (warp + 1) / warps : e0;
+    Key2* list = lists[warp];
+    Key2 floor{0, 0};
+    int cnt = 0;
+    int64_t e = e0;
+    int b0 = warp == 0 && finished ? 0 : beams;
+    while (true) {
+      const bool more = e < e1 || b0 < beams;
+      if (cnt > kCap - kWarp || (!more && cnt)) {
+        sort_some<LONG>(list, cnt, keep, lane, [&](int i) { return list[i]; });
+        cnt = min(cnt, keep);
+        if (cnt == keep) floor = list[keep - 1];
+      }
+      if (!more) break;
+      bool take = false;
+      Key2 k{0, 0};
+      if (e < e1) {
+        const int64_t at = e + lane;
+        if (at < e1) {
+          const int b = small ? static_cast<int>(static_cast<uint32_t>(at) / static_cast<uint32_t>(per_beam))
+                              : static_cast<int>(at / per_beam);
+          if (kind[b] == 1) {   // rows without candidates have no lists
+            const uint64_t x = cand[g * total + at].a;
+            take = x != 0;
+            if (take)
+              k = {ord64(offs[b] + (static_cast<double>(unord32(static_cast<uint32_t>(x >> 32))) - tops[b])),
+                   ~(static_cast<uint32_t>(b) * vocab + ~static_cast<uint32_t>(x))};
+          }
+        }
+        e += kWarp;
+      } else {
+        const int b = b0 + lane;
+        take = b < beams && kind[b] == 2;
+        if (take) k = {ord64(static_cast<double>(sc[b])), ~(static_cast<uint32_t>(b) * vocab + end_token)};
+        b0 += kWarp;
+      }
       take = take && k.above(floor);
       const unsigned pass = __ballot_sync(kFull, take);
       if (take) list[cnt + __popc(pass & ((1u << lane) - 1u))] = k;
       cnt += __popc(pass);
     }
-  }
-  if (cnt) cut();
-  const int nkept = cnt;
-  for (int j = lane; j < keep; j += kWarp) {
-    const bool ok = j < nkept;
-    const Key2 k = ok ? list[j] : Key2{0, 0};
-    const uint32_t idx = ~k.b, b = ok ? idx / static_cast<uint32_t>(vocab) : 0u;
-    out_s[g * keep + j] = ok ? static_cast<float>(unord64(k.a)) : -INFINITY;
-    out_p[g * keep + j] = ok ? static_cast<int32_t>(b) : -1;
-    out_t[g * keep + j] = ok ? static_cast<int32_t>(idx - b * vocab) : -1;
-  }
-}
-
-// --------------------------------------------------- one block, many rows
-// Selection among elements of several rows, each held as f = fl32(x + c_b)
-// in registers (NaN: no candidate), c_b the row's offset rounded to float32.
-// f is within 2^-24 (|c_b| + |f|) of the exact value v, so with F the keep-th
-// largest f (or a lower bound of it) every kept candidate has
-// f >= F - 2^-22 (max |c_b| + |F|): those are gathered, valued in 64 bits and
-// sorted.
-struct Picked {
-  double v[kBeamMax];
-  uint32_t i[kBeamMax];
-  int n;
-};
-
-struct SelShared {
-  double off[kBeamMax];     // S_b, less the log of the row's sum
-  float top[kBeamMax];      // the row's maximum (log-softmax), else 0
-  float c[kBeamMax];        // off - top, NaN for a row without elements
-  uint8_t fin[kBeamMax];
-  float cmax;
-  uint32_t rth[8], hi[8];
-  int red[8], count;
-  uint32_t hits[kHits];     // element, or kHitFinished + beam, or kHitKept + slot
-  Picked kept;
-  double rv[8];
-  uint32_t ri[8];
-  double lv;
-  uint32_t li;
-};
-constexpr uint32_t kHitFinished = 0xc0000000u, kHitKept = 0xd0000000u;
-
-// offsets of the rows; SUM gives a row's maximum and sum of exponentials
-__device__ __forceinline__ void set_row(SelShared& sh, int b, float score, bool fin, bool softmax, float mx,
-                                        double sum) {
-  const bool ok = live(score);
-  sh.fin[b] = ok && fin;
-  sh.off[b] = static_cast<double>(score) - (softmax && sum > 0.0 ? log(sum) : 0.0);
-  sh.top[b] = softmax && fabsf(mx) < INFINITY ? mx : 0.f;
-  sh.c[b] = ok && !fin ? static_cast<float>(sh.off[b] - static_cast<double>(sh.top[b])) : kNan;
-}
-
-__device__ __forceinline__ double row_value(const SelShared& sh, int b, float x) {
-  return sh.off[b] + (static_cast<double>(x) - static_cast<double>(sh.top[b]));
-}
-
-// Src: f[E] a thread, and exact(i, v, idx) for the thread's i-th element.
-// Elements are named by name(i); `value(name, v, idx)` gives any element's
-// exact value. The result is left in sh.kept, sorted.
-template <int NW, int E, typename Name, typename Value>
-__device__ __forceinline__ void block_select(SelShared& sh, const float (&f)[E], int beams, int vocab, int keep,
-                                             int end_token, bool first, Name&& name, Value&& value,
-                                             const float* __restrict__ scores) {
-  constexpr int NT = NW * kWarp;
-  const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
-  const int r = (keep + NW - 1) / NW;
-  float mx = kNan;
+    if (lane == 0) counts[warp] = cnt;
+    __syncthreads();
+    int found = 0;
 #pragma unroll
-  for (int i = 0; i < E; ++i) mx = fmaxf(mx, f[i]);
-  const uint32_t u = isnan(mx) ? 0u : ord32(mx);
-  const uint32_t wm = __reduce_max_sync(kFull, u), wr = r <= kWarp ? warp_rth(u, r, lane) : 0u;
-  if (lane == 0) {
-    sh.rth[warp] = wr;
-    sh.hi[warp] = wm;
-  }
-  if (tid == 0) sh.count = 0;
-  __syncthreads();
-  uint32_t lo = sh.rth[0], hi = sh.hi[0];
-#pragma unroll
-  for (int w = 1; w < NW; ++w) {
-    lo = min(lo, sh.rth[w]);
-    hi = max(hi, sh.hi[w]);
-  }
-  const int kept = first ? 0 : sh.kept.n;
-  // what is kept from the tiles before bounds this one from below
-  float carry = -INFINITY;
-  if (kept == keep) carry = static_cast<float>(sh.kept.v[keep - 1]);
-  auto at_least = [&](uint32_t k) {
-    const float t = unord32(k);
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < E; ++i) n += f[i] >= t;
-    return block_sum<NW>(n, sh.red);
-  };
-  auto threshold = [&](uint32_t k) {
-    const float t = fmaxf(k ? unord32(k) : -INFINITY, carry);
-    const float thr = t - 0x1p-22f * (sh.cmax + fabsf(t));
-    return isnan(thr) ? -INFINITY : thr;
-  };
-  auto collect = [&](float thr) {
-#pragma unroll
-    for (int i = 0; i < E; ++i)
-      if (f[i] >= thr) {
-        const int at = atomicAdd(&sh.count, 1);
-        if (at < kHits) sh.hits[at] = name(i);
-      }
-    if (first)
-      for (int b = tid; b < beams; b += NT)
-        if (sh.fin[b] && scores[b] >= thr) {
-          const int at = atomicAdd(&sh.count, 1);
-          if (at < kHits) sh.hits[at] = kHitFinished + b;
+    for (int w = 0; w < kMergeWarps; ++w) found += counts[w];
+    for (int j = tid; j < kMergeWarps * keep; j += kMergeWarps * kWarp) {
+      const int w = j / keep, i = j - w * keep;
+      if (i >= counts[w]) continue;
+      const Key2 k = lists[w][i];
+      int rank = i;
+      for (int o = 0; o < warps; ++o) {
+        if (o == w) continue;
+        int lo = 0, hi = counts[o];   // keys above k come first
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if (lists[o][mid].above(k)) lo = mid + 1;
+          else hi = mid;
         }
-    for (int j = tid; j < kept; j += NT)
-      if (sh.kept.v[j] >= static_cast<double>(thr)) {
-        const int at = atomicAdd(&sh.count, 1);
-        if (at < kHits) sh.hits[at] = kHitKept + j;
+        rank += lo;
       }
-  };
-  // fewer survivors are cheaper to sort: bisect while there are more than the
-  // power of two that holds `keep`
-  int limit = 32;
-  while (limit < keep) limit <<= 1;
-  int rounds = keep > 32 ? 8 : 0, c;
-  bool all = false;
-  if (rounds && lo && at_least(lo) <= limit) rounds = 0;
-  while (true) {
-    uint32_t up = hi + 1;
-    for (; rounds > 0 && up - lo > 1; --rounds) {
-      const uint32_t mid = lo + (up - lo) / 2;
-      const int n = at_least(mid);
-      if (n >= keep) {
-        lo = mid;
-        if (n <= limit) break;
-      } else {
-        up = mid;
+      if (rank < keep) {
+        const uint32_t idx = ~k.b, b = idx / static_cast<uint32_t>(vocab);
+        out_s[g * keep + rank] = static_cast<float>(unord64(k.a));
+        out_p[g * keep + rank] = static_cast<int32_t>(b);
+        out_t[g * keep + rank] = static_cast<int32_t>(idx - b * vocab);
       }
     }
-    collect(threshold(lo));
-    __syncthreads();
-    c = sh.count;
-    if (c <= kHits || all) break;
-    __syncthreads();
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
-    rounds = 34;
-    all = true;
-  }
-  auto exact = [&](uint32_t h, double& v, uint32_t& idx) {
-    if (h >= kHitKept) {
-      v = sh.kept.v[h - kHitKept];
-      idx = sh.kept.i[h - kHitKept];
-    } else if (h >= kHitFinished) {
-      const int b = h - kHitFinished;
-      v = static_cast<double>(scores[b]);
-      idx = static_cast<uint32_t>(b) * vocab + end_token;
-    } else {
-      value(h, v, idx);
+    for (int j = found + tid; j < keep; j += kMergeWarps * kWarp) {
+      out_s[g * keep + j] = -INFINITY;
+      out_p[g * keep + j] = -1;
+      out_t[g * keep + j] = -1;
     }
-  };
-  if (c <= kHits) {
-    if (warp == 0) {
-      auto sorted = [&](auto tag) {
-        constexpr int P = decltype(tag)::value;
-        Key2 k[P];
-#pragma unroll
-        for (int n = 0; n < P; ++n) {
-          k[n] = {0, 0};
-          if (n * kWarp + lane < c) {
-            double v;
-            uint32_t idx;
-            exact(sh.hits[n * kWarp + lane], v, idx);
-            k[n] = {ord64(v), ~idx};
-          }
-        }
-        __syncwarp();
-        warp_sort<P>(k, lane);
-#pragma unroll
-        for (int n = 0; n < P; ++n)
-          if (n * kWarp + lane < keep) {
-            sh.kept.v[n * kWarp + lane] = unord64(k[n].a);
-            sh.kept.i[n * kWarp + lane] = ~k[n].b;
-          }
-      };
-      if (c <= 32) sorted(std::integral_constant<int, 1>{});
-      else if (c <= 64) sorted(std::integral_constant<int, 2>{});
-      else if (c <= 128) sorted(std::integral_constant<int, 4>{});
-      else sorted(std::integral_constant<int, 8>{});
-      if (lane == 0) sh.kept.n = min(c, keep);
-    }
-    __syncthreads();
-    return;
-  }
-  // Many equal values: one kept candidate a round, the best behind the last.
-  // Results go to the hit list's place only when all are found, because the
-  // kept ones of earlier tiles take part.
-  double pv = INFINITY, tv[(kBeamMax + NT - 1) / NT];
-  uint32_t pi = 0, ti[(kBeamMax + NT - 1) / NT];
-  int found = 0;
-  for (int j = 0; j < keep; ++j) {
-    double v = -INFINITY;
-    uint32_t vi = 0xffffffffu;
-    auto offer = [&](double x, uint32_t idx) {
-      if (j > 0 && (x > pv || (x == pv && idx <= pi))) return;
-      if (vi == 0xffffffffu || x > v || (x == v && idx < vi)) {
-        v = x;
-        vi = idx;
-      }
-    };
-    const float thr = threshold(lo);
-#pragma unroll
-    for (int i = 0; i < E; ++i)
-      if (f[i] >= thr) {
-        double x;
-        uint32_t idx;
-        value(name(i), x, idx);
-        offer(x, idx);
-      }
-    if (first)
-      for (int b = tid; b < beams; b += NT)
-        if (sh.fin[b]) offer(static_cast<double>(scores[b]), static_cast<uint32_t>(b) * vocab + end_token);
-    for (int q = tid; q < kept; q += NT) offer(sh.kept.v[q], sh.kept.i[q]);
-    auto join = [&](double v2, uint32_t i2) {
-      if (i2 != 0xffffffffu && (vi == 0xffffffffu || v2 > v || (v2 == v && i2 < vi))) {
-        v = v2;
-        vi = i2;
-      }
-    };
-    for (int o = 16; o; o >>= 1) {
-      const double v2 = __shfl_xor_sync(kFull, v, o);
-      const uint32_t i2 = __shfl_xor_sync(kFull, vi, o);
-      join(v2, i2);
-    }
-    if (lane == 0) {
-      sh.rv[warp] = v;
-      sh.ri[warp] = vi;
-    }
-    __syncthreads();
-    v = -INFINITY;
-    vi = 0xffffffffu;
-    for (int w = 0; w < NW; ++w) join(sh.rv[w], sh.ri[w]);
-    __syncthreads();
-    if (vi == 0xffffffffu) break;
-    pv = v;
-    pi = vi;
-    if (j % NT == tid) {
-#pragma unroll
-      for (int q = 0; q < (kBeamMax + NT - 1) / NT; ++q)
-        if (q == j / NT) {
-          tv[q] = v;
-          ti[q] = vi;
-        }
-    }
-    found = j + 1;
-  }
-#pragma unroll
-  for (int q = 0; q < (kBeamMax + NT - 1) / NT; ++q)
-    if (q * NT + tid < found) {
-      sh.kept.v[q * NT + tid] = tv[q];
-      sh.kept.i[q * NT + tid] = ti[q];
-    }
-  if (tid == 0) sh.kept.n = found;
-  __syncthreads();
-}
-
-template <int NW>
-__device__ __forceinline__ void write_kept(const SelShared& sh, int64_t g, int vocab, int keep,
-                                           float* __restrict__ out_s, int32_t* __restrict__ out_p,
-                                           int32_t* __restrict__ out_t) {
-  for (int j = threadIdx.x; j < keep; j += NW * kWarp) {
-    const bool ok = j < sh.kept.n;
-    const uint32_t idx = ok ? sh.kept.i[j] : 0u, b = idx / static_cast<uint32_t>(vocab);
-    out_s[g * keep + j] = ok ? static_cast<float>(sh.kept.v[j]) : -INFINITY;
-    out_p[g * keep + j] = ok ? static_cast<int32_t>(b) : -1;
-    out_t[g * keep + j] = ok ? static_cast<int32_t>(idx - b * vocab) : -1;
-  }
-}
-
-// the largest finite |c_b|: what c's own rounding can be off by
-__device__ __forceinline__ void set_cmax(SelShared& sh, int beams) {
-  if (threadIdx.x < kWarp) {
-    float m = 0.f;
-    for (int b = threadIdx.x; b < beams; b += kWarp) m = fmaxf(m, fabsf(sh.c[b]));
-    m = __uint_as_float(__reduce_max_sync(kFull, __float_as_uint(m)));
-    if (threadIdx.x == 0) sh.cmax = m;
-  }
-}
-
-// The segments' candidates of one group joined: one block a group, tiles of
-// 32 x 8 x 16 candidates.
-constexpr int kMergeWarps = 8, kMergeElems = 16;
-
-__global__ void __launch_bounds__(kMergeWarps* kWarp) merge_kernel(
-    const Key1* __restrict__ cand, const SegStat* __restrict__ stats, const float* __restrict__ scores,
-    const uint8_t* __restrict__ finished, int64_t groups, int beams, int vocab, int keep, int segs, int softmax,
-    int end_token, float* __restrict__ out_s, int32_t* __restrict__ out_p, int32_t* __restrict__ out_t) {
-  constexpr int NT = kMergeWarps * kWarp, E = kMergeElems;
-  __shared__ SelShared sh;
-  const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
-  cudaGridDependencySynchronize();
-  const int64_t per_beam = static_cast<int64_t>(segs) * keep, total = per_beam * beams;
-  for (int64_t g = blockIdx.x; g < groups; g += gridDim.x) {
-    const float* sc = scores + g * beams;
-    for (int b = warp; b < beams; b += kMergeWarps) {
-      const bool fin = finished && finished[g * beams + b];
-      double mx = -INFINITY, sum = 0.0;
-      if (softmax && !fin && live(sc[b])) {
-        const SegStat* st = stats + (g * beams + b) * segs;
-        for (int s = lane; s < segs; s += kWarp) mx = fmax(mx, st[s].max);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) mx = fmax(mx, __shfl_xor_sync(kFull, mx, o));
-        if (mx > -INFINITY)
-          for (int s = lane; s < segs; s += kWarp)
-            if (st[s].sum > 0.0) sum += st[s].sum * exp(st[s].max - mx);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-      }
-      if (lane == 0) set_row(sh, b, sc[b], fin, softmax, static_cast<float>(mx), sum);
-    }
-    __syncthreads();
-    set_cmax(sh, beams);
-    const Key1* list = cand + g * total;
-    for (int64_t t0 = 0; t0 < total; t0 += NT * E) {
-      float f[E];
-      auto name = [&](int i) { return static_cast<uint32_t>(i * NT + tid); };
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const int64_t e = t0 + i * NT + tid;
-        f[i] = kNan;
-        if (e < total) {
-          const float c = sh.c[e / per_beam];
-          if (!isnan(c)) {   // rows without candidates have no lists
-            const uint64_t k = list[e].a;
-            if (k) f[i] = __fadd_rn(unord32(static_cast<uint32_t>(k >> 32)), c);
-          }
-        }
-      }
-      auto value = [&](uint32_t e, double& v, uint32_t& idx) {
-        const uint64_t k = list[t0 + e].a;
-        const int b = static_cast<int>((t0 + e) / per_beam);
-        v = row_value(sh, b, unord32(static_cast<uint32_t>(k >> 32)));
-        idx = static_cast<uint32_t>(b) * vocab + ~static_cast<uint32_t>(k);
-      };
-      block_select<kMergeWarps, E>(sh, f, beams, vocab, keep, end_token, t0 == 0, name, value, sc);
-    }
-    write_kept<kMergeWarps>(sh, g, vocab, keep, out_s, out_p, out_t);
     __syncthreads();
   }
 }
@@ -1068,10 +891,11 @@ cudaError_t run_group(const SelectArgs& a, cudaStream_t st) {
   };
   const bool many = a.keep > kShortKeep;
   if (!vec) return many ? run(group_kernel<T, 1, 16, true>) : run(group_kernel<T, 1, 16, false>);
-  if (many) return run(group_kernel<T, n, 32, true>);
-  const int64_t total = static_cast<int64_t>(a.beams) * a.vocab;
-  return total > 32 * kWarp && total <= 64 * kWarp ? run(group_kernel<T, n, 64, false>)
-                                                    : run(group_kernel<T, n, 32, false>);
+  // 16 vectors a lane when they hold the whole group
+  const int64_t nvec = static_cast<int64_t>(div) * a.beams;
+  if (nvec > 8 * kWarp && nvec <= 16 * kWarp)
+    return many ? run(group_kernel<T, n, 16, true>) : run(group_kernel<T, n, 16, false>);
+  return many ? run(group_kernel<T, n, 8, true>) : run(group_kernel<T, n, 8, false>);
 }
 
 template <typename T>
@@ -1102,9 +926,9 @@ cudaError_t run_split(const SelectArgs& a, const SelectPlan& p, int sm_count, cu
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, merge_kernel, static_cast<const Key1*>(cand), static_cast<const SegStat*>(stats),
-                            a.scores, a.finished, a.groups, a.beams, a.vocab, a.keep, p.segs, a.softmax, a.end_token,
-                            a.out_scores, a.out_parents, a.out_tokens);
+  return cudaLaunchKernelEx(&cfg, many ? merge_kernel<true> : merge_kernel<false>, static_cast<const Key1*>(cand),
+                            static_cast<const SegStat*>(stats), a.scores, a.finished, a.groups, a.beams, a.vocab,
+                            a.keep, p.segs, a.softmax, a.end_token, a.out_scores, a.out_parents, a.out_tokens);
 }
 
 template <typename T>

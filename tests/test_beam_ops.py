@@ -12,14 +12,12 @@ from gustann_b200.api import GustANNError, beam_select, matmul_i8, quantize_rows
 DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 
 
-def ref_select(scores, logits, k, softmax=False, finished=None, end=0):
+def ref_values(scores, logits, softmax=False, finished=None, end=0):
+    """Every candidate's value in 64 bits, [g, w * v]; -inf where there is none."""
     lg = logits.cpu().double().numpy()
     sc = scores.cpu().double().numpy()
     g, w, v = lg.shape
-    val = np.full((g, k), -np.inf)
-    par = np.full((g, k), -1)
-    tok = np.full((g, k), -1)
-    flat = np.arange(w * v)
+    out = np.empty((g, w * v))
     for i in range(g):
         c = np.where(np.isfinite(lg[i]), lg[i], -np.inf)
         if softmax:
@@ -32,25 +30,61 @@ def ref_select(scores, logits, k, softmax=False, finished=None, end=0):
             for b in np.flatnonzero(finished[i].cpu().numpy()):
                 c[b] = -np.inf
                 c[b, end] = 0
-        c = np.where(np.isfinite(sc[i])[:, None], c + np.where(np.isfinite(sc[i]), sc[i], 0)[:, None], -np.inf).ravel()
-        o = np.lexsort((flat, -c))[:k]
-        o = o[np.isfinite(c[o])]
-        val[i, :o.size], par[i, :o.size], tok[i, :o.size] = c[o], o // v, o % v
+        out[i] = np.where(np.isfinite(sc[i])[:, None], c + np.where(np.isfinite(sc[i]), sc[i], 0)[:, None],
+                          -np.inf).ravel()
+    return out
+
+
+def ref_select(scores, logits, k, softmax=False, finished=None, end=0, values=None):
+    c = ref_values(scores, logits, softmax, finished, end) if values is None else values
+    g, v = c.shape[0], logits.shape[2]
+    val = np.full((g, k), -np.inf)
+    par = np.full((g, k), -1)
+    tok = np.full((g, k), -1)
+    for i in range(g):
+        o = np.lexsort((np.arange(c.shape[1]), -c[i]))[:k]
+        o = o[np.isfinite(c[i, o])]
+        val[i, :o.size], par[i, :o.size], tok[i, :o.size] = c[i, o], o // v, o % v
     return val, par, tok
 
 
+# with log-softmax the sum of exponentials is off by 2^-22 (2 steps of the
+# exponential), 2^-24 times the arguments (at most log of the vocabulary, 21,
+# on the sum's average; the constant log2 e and the step's rounding, one each)
+# and at most 64 sums in float32: below 2^-17 together, which is the logarithm's
+# error, one and the same for all candidates of a row
+LSE = 2.0 ** -17
+
+
 def check_select(scores, logits, k, softmax=False, finished=None, end=0):
-    s, p, t = beam_select(scores, logits, k, log_softmax=softmax, finished=finished, end_token=end)
-    rv, rp, rt = ref_select(scores, logits, k, softmax, finished, end)
-    assert np.array_equal(p.cpu().numpy(), rp)
-    assert np.array_equal(t.cpu().numpy(), rt)
-    s = s.cpu().double().numpy()
-    # the 64-bit value rounded to float32; with log-softmax the sum of
-    # exponentials is off by 2^-22 (2 steps of expf), 2^-24 times the arguments
-    # (at most log of the vocabulary, 21, on the sum's average) and at most 64
-    # sums in float32: below 2^-17 together, which is the logarithm's error
+    s, p, t = (x.cpu().numpy() for x in
+               beam_select(scores, logits, k, log_softmax=softmax, finished=finished, end_token=end))
+    values = ref_values(scores, logits, softmax, finished, end)
+    rv, rp, rt = ref_select(scores, logits, k, softmax, finished, end, values)
+    v = logits.shape[2]
+    if softmax:
+        # Rows' values are off by LSE at most, so the i-th best by the computed
+        # values is within 2 LSE of the i-th best by the exact ones, and only
+        # candidates of different rows that near to each other can trade places:
+        # as many candidates, none twice, and each row's in exact order.
+        assert np.array_equal(p < 0, rp < 0) and np.array_equal(t < 0, rt < 0)
+        for i in range(len(p)):
+            n = int((p[i] >= 0).sum())
+            flat = p[i, :n].astype(np.int64) * v + t[i, :n]
+            assert len(set(flat.tolist())) == n
+            with np.errstate(invalid="ignore"):
+                assert bool((np.abs(values[i, flat] - rv[i, :n]) <= 2 * LSE).all())
+            for b in set(p[i, :n].tolist()):
+                f = flat[p[i, :n] == b]
+                row = np.lexsort((np.arange(v), -values[i, b * v:(b + 1) * v]))[:f.size]
+                assert np.array_equal(f - b * v, row)
+            rv[i, :n] = values[i, flat]
+    else:
+        assert np.array_equal(p, rp) and np.array_equal(t, rt)
+    s = s.astype(np.float64)
+    # the 64-bit value rounded to float32
     with np.errstate(invalid="ignore"):
-        bound = 2.0 ** -24 * np.abs(rv) * 1.01 + (2.0 ** -17 if softmax else 0.0)
+        bound = 2.0 ** -24 * np.abs(rv) * 1.01 + (LSE if softmax else 0.0)
         lost = np.abs(rv) > np.finfo(np.float32).max
         assert bool(((np.abs(s - rv) <= bound) | (s == rv) | (lost & np.isinf(s))).all())
 
