@@ -202,6 +202,107 @@ __device__ __forceinline__ float i8_value(int acc, float sa, float sb, float bia
   return __fmaf_rn(static_cast<float>(acc) * sa, sb, bias);
 }
 
+// ------------------------------------------------------------ one to four rows
+// With one to four rows of a the product only reads b: bound by memory, dp4a
+// keeps up with it. A group of `lanes` lanes (as few as its vectors of 16 codes
+// need, at least 8) takes R rows of b at a time, so a's vector is read from
+// shared memory once for R of b's and R loads are on their way; the R sums are
+// folded into the lanes while they are added up.
+constexpr int kThinRows = 4, kThinThreads = 256, kThinBytes = 48 * 1024;
+
+__device__ __forceinline__ int dot16(const uint4& x, const uint4& y, int acc) {
+  acc = __dp4a(static_cast<int>(x.x), static_cast<int>(y.x), acc);
+  acc = __dp4a(static_cast<int>(x.y), static_cast<int>(y.y), acc);
+  acc = __dp4a(static_cast<int>(x.z), static_cast<int>(y.z), acc);
+  return __dp4a(static_cast<int>(x.w), static_cast<int>(y.w), acc);
+}
+
+template <typename T, int M, int R>
+__global__ void __launch_bounds__(kThinThreads) thin_kernel(const int8_t* __restrict__ a, int m, int64_t as,
+                                                            const float* __restrict__ sa, const int8_t* __restrict__ b,
+                                                            int64_t n, int64_t bs, const float* __restrict__ sb,
+                                                            const float* __restrict__ bias, int k, int lanes,
+                                                            T* __restrict__ out, int64_t os) {
+  extern __shared__ uint4 rows_a[];   // [M][nv], zeros past k and m
+  const int nv = (k + 15) / 16, tid = threadIdx.x;
+  for (int e = tid; e < M * nv; e += kThinThreads) {
+    const int i = e / nv, v = e - i * nv;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (i < m) {
+      const int8_t* p = a + i * as + v * 16;
+      if (v * 16 + 16 <= k) {
+        w = *reinterpret_cast<const uint4*>(p);
+      } else {
+        uint32_t q[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (v * 16 + j < k) q[j / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(p[j])) << (8 * (j % 4));
+        w = make_uint4(q[0], q[1], q[2], q[3]);
+      }
+    }
+    rows_a[e] = w;
+  }
+  __syncthreads();
+  const int lane = tid & (lanes - 1);
+  const int64_t per = kThinThreads / lanes, groups = (n + R - 1) / R;
+  // every lane of a warp takes part in the folding, so loops run whole
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * per;
+  for (int64_t q0 = first; q0 < groups; q0 += static_cast<int64_t>(gridDim.x) * per) {
+    const int64_t r0 = (q0 + tid / lanes) * R;
+    int acc[M][R];
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+      for (int r = 0; r < R; ++r) acc[i][r] = 0;
+#pragma unroll(R == 1 ? 4 : 2)
+    for (int v = lane; v < nv; v += lanes) {
+      uint4 w[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int64_t row = min(r0 + r, n - 1);
+        const int8_t* p = b + row * bs + static_cast<int64_t>(v) * 16;
+        // the last vector's codes past k meet zeros; behind the last row there
+        // may be no memory for them
+        if (v * 16 + 16 <= k || row < n - 1) {
+          w[r] = __ldcs(reinterpret_cast<const uint4*>(p));
+        } else {
+          uint32_t z[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (v * 16 + j < k) z[j / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(p[j])) << (8 * (j % 4));
+          w[r] = make_uint4(z[0], z[1], z[2], z[3]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        const uint4 x = rows_a[i * nv + v];
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[i][r] = dot16(w[r], x, acc[i][r]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      int sum;
+      int64_t row = r0;
+      if (R == 4) {
+        // lanes 0..3 of every four end up with rows 0..3
+        const bool hi = lane & 2, odd = lane & 1;
+        const int x0 = hi ? acc[i][2 % R] : acc[i][0], y0 = hi ? acc[i][0] : acc[i][2 % R];
+        const int x1 = hi ? acc[i][3 % R] : acc[i][1 % R], y1 = hi ? acc[i][1 % R] : acc[i][3 % R];
+        const int s0 = x0 + __shfl_xor_sync(kFull, y0, 2), s1 = x1 + __shfl_xor_sync(kFull, y1, 2);
+        sum = (odd ? s1 : s0) + __shfl_xor_sync(kFull, odd ? s0 : s1, 1);
+        for (int o = 4; o < lanes; o <<= 1) sum += __shfl_xor_sync(kFull, sum, o);
+        row += lane & 3;
+      } else {
+        sum = acc[i][0];
+        for (int o = 1; o < lanes; o <<= 1) sum += __shfl_xor_sync(kFull, sum, o);
+      }
+      if (lane < R && row < n && i < m)
+        out[i * os + row] = from_f32<T>(i8_value(sum, sa[i], sb[row], bias ? bias[row] : 0.f));
+    }
+  }
+}
+
 // ------------------------------------------------------- tensor-core product
 // The 5th-generation tensor cores multiply signed bytes with 32-bit sums
 // (tcgen05.mma, kind::i8): 128 rows of b by `tn` rows of a, 128 bytes of k a
@@ -740,6 +841,29 @@ cudaError_t launch_quantize_rows(const void* x, int64_t rows, int64_t stride, in
 
 namespace {
 
+// Rows of a that the kernel is made for: 1, 2 or 4.
+int thin_rows(int64_t m) { return m <= 2 ? static_cast<int>(m) : 4; }
+
+// Four rows of b at a time when that leaves 16 warps and more for every SM.
+template <typename T>
+cudaError_t run_thin(const int8_t* a, int64_t m, int64_t as, const float* sa, const int8_t* b, int64_t n, int64_t bs,
+                     const float* sb, const float* bias, int k, T* out, int64_t os, int sm_count, cudaStream_t st) {
+  const int nv = (k + 15) / 16;
+  const int lanes = nv <= 16 ? 8 : nv <= 64 ? 16 : 32;
+  const bool four = n * lanes / 4 >= static_cast<int64_t>(sm_count) * 16 * kWarp;
+  const size_t smem = static_cast<size_t>(thin_rows(m)) * nv * 16;
+  auto run = [&](auto fn, int r) {
+    const int64_t per = kThinThreads / lanes * r;
+    const int64_t grid = std::min<int64_t>((n + per - 1) / per, static_cast<int64_t>(sm_count) * 8);
+    fn<<<static_cast<unsigned>(grid), kThinThreads, smem, st>>>(a, static_cast<int>(m), as, sa, b, n, bs, sb, bias, k,
+                                                                lanes, out, os);
+    return cudaGetLastError();
+  };
+  if (m == 1) return four ? run(thin_kernel<T, 1, 4>, 4) : run(thin_kernel<T, 1, 1>, 1);
+  if (m == 2) return four ? run(thin_kernel<T, 2, 4>, 4) : run(thin_kernel<T, 2, 1>, 1);
+  return four ? run(thin_kernel<T, 4, 4>, 4) : run(thin_kernel<T, 4, 1>, 1);
+}
+
 // cuTensorMapEncodeTiled from the driver that the runtime has loaded.
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -797,6 +921,11 @@ cudaError_t launch_matmul_i8(const int8_t* a, int64_t m, int64_t as, const float
                              int64_t bs, const float* sb, const float* bias, int k, void* out, int64_t os, int dtype,
                              int sm_count, cudaStream_t st) {
   if (m <= 0 || n <= 0) return cudaSuccess;
+  if (m <= kThinRows && thin_rows(m) * ((k + 15) / 16) * 16 <= kThinBytes) {
+    if (dtype == GANN_F32) return run_thin(a, m, as, sa, b, n, bs, sb, bias, k, static_cast<float*>(out), os, sm_count, st);
+    if (dtype == GANN_F16) return run_thin(a, m, as, sa, b, n, bs, sb, bias, k, static_cast<__half*>(out), os, sm_count, st);
+    return run_thin(a, m, as, sa, b, n, bs, sb, bias, k, static_cast<__nv_bfloat16*>(out), os, sm_count, st);
+  }
   const MmaPlan plan = plan_mma(m, n, k, sm_count);
   MmaArgs p{};
   p.sa = sa;

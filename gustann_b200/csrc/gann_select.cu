@@ -198,6 +198,51 @@ __device__ __forceinline__ void sort_some(K* kept, int total, int keep, int lane
   else if (total <= 128) sort_keys<4>(kept, total, keep, lane, get);
   else sort_keys<8>(kept, total, keep, lane, get);
 }
+// More than 128 (float, index) keys of which at most 128 are kept: the floats'
+// order is bisected until between `keep` and 128 keys pass, which halves the
+// sort. Returns how many are left, all of them if equal floats leave no such
+// place.
+__device__ __forceinline__ int trim_long(Key1* list, int total, int keep, int lane) {
+  Key1 k[kHits / kWarp];
+  uint32_t lo = 0xffffffffu, hi = 0;
+  __syncwarp();
+#pragma unroll
+  for (int n = 0; n < kHits / kWarp; ++n) {
+    k[n] = n * kWarp + lane < total ? list[n * kWarp + lane] : Key1{0};
+    if (k[n].a) {
+      lo = min(lo, static_cast<uint32_t>(k[n].a >> 32));
+      hi = max(hi, static_cast<uint32_t>(k[n].a >> 32));
+    }
+  }
+  lo = __reduce_min_sync(kFull, lo);
+  hi = __reduce_max_sync(kFull, hi) + 1;
+  int n_lo = total;
+  while (n_lo > 128 && hi - lo > 1) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    int c = 0;
+#pragma unroll
+    for (int n = 0; n < kHits / kWarp; ++n) c += static_cast<uint32_t>(k[n].a >> 32) >= mid;
+    c = __reduce_add_sync(kFull, c);
+    if (c >= keep) {
+      lo = mid;
+      n_lo = c;
+    } else {
+      hi = mid;
+    }
+  }
+  if (n_lo > 128) return total;
+  int at = 0;
+#pragma unroll
+  for (int n = 0; n < kHits / kWarp; ++n) {
+    const bool take = k[n].a && static_cast<uint32_t>(k[n].a >> 32) >= lo;
+    const unsigned m = __ballot_sync(kFull, take);
+    if (take) list[at + __popc(m & ((1u << lane) - 1u))] = k[n];
+    at += __popc(m);
+  }
+  __syncwarp();
+  return at;
+}
+
 // Candidates that a warp holds at a time, kept ones among them, in the two
 // forms of the kernels below: keep <= 16, and more.
 constexpr int kShortKeep = 16;
@@ -276,6 +321,7 @@ __global__ void __launch_bounds__(kRowWarps* kWarp, 5) row_kernel(const T* __res
   int cnt = 0;
   float thr = -INFINITY, m = -INFINITY, m2 = 0.f, fix = 1.f;
   auto cut = [&]() {
+    if (LONG && cnt > 128) cnt = trim_long(list, cnt, keep, lane);
     sort_some<LONG>(list, cnt, keep, lane, [&](int i) { return list[i]; });
     cnt = min(cnt, keep);
     if (cnt < keep) return;
@@ -485,7 +531,7 @@ __global__ void __launch_bounds__(kGroupWarps* kWarp, NV * VW > 32 ? 5 : 7) grou
     return static_cast<double>(c[b]) + static_cast<double>(Raw<T>::one(base + b * bstride + (id - b * vocab)));
   };
   auto cut = [&]() {
-    const int total = cnt;
+    const int total = LONG && cnt > 128 ? trim_long(list, cnt, keep, lane) : cnt;
     sort_some<LONG>(list, total, total, lane, [&](int i) { return list[i]; });
     bool equal = false;
     for (int i = lane; i + 1 < total && i < keep; i += kWarp) equal |= (list[i].a >> 32) == (list[i + 1].a >> 32);
