@@ -11,6 +11,7 @@ is no fallback: if it is missing, importing this module raises.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 from dataclasses import dataclass
 
@@ -592,6 +593,13 @@ def matmul_i8(a, a_scales, b, b_scales, bias=None, dtype=None, out=None, stream:
     return out
 
 
+@functools.lru_cache(maxsize=1024)
+def _select_workspace(g, w, v, k, dt, soft) -> int:
+    need = C.c_int64()
+    _check(lib.gann_beam_select_workspace(g, w, v, k, dt, soft, C.byref(need)))
+    return need.value
+
+
 def beam_select(scores, logits, k: int, log_softmax: bool = False, finished=None, end_token: int = 0,
                 stream: int | None = None):
     """The best ``k`` continuations of each group's beams (``gann_beam_select``):
@@ -622,19 +630,18 @@ def beam_select(scores, logits, k: int, log_softmax: bool = False, finished=None
         with _stream_scope(dev, stream):
             return beam_select(scores, logits, k, log_softmax, finished, end_token)
     soft = 1 if log_softmax else 0
-    need = C.c_int64()
-    _check(lib.gann_beam_select_workspace(g, w, v, k, dt, soft, C.byref(need)))
+    need = _select_workspace(g, w, v, k, dt, soft)
     scores = scores.contiguous()
     if finished is not None:
         finished = finished.contiguous()
-    ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     out_s = torch.empty(g, k, dtype=torch.float32, device=dev)
     out_p = torch.empty(g, k, dtype=torch.int32, device=dev)
     out_t = torch.empty_like(out_p)
     _check(lib.gann_beam_select(logits.data_ptr(), dt, gs, bs, scores.data_ptr(),
                                 None if finished is None else finished.data_ptr(), g, w, v, k, soft, end_token,
                                 out_s.data_ptr(), out_p.data_ptr(), out_t.data_ptr(),
-                                None if ws is None else ws.data_ptr(), need.value, index,
+                                None if ws is None else ws.data_ptr(), need, index,
                                 torch._C._cuda_getCurrentRawStream(index)))
     return out_s, out_p, out_t
 

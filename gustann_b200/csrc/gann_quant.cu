@@ -561,6 +561,40 @@ __global__ void __launch_bounds__(kMmaThreads, 1) mma_kernel(const __grid_consta
   int columns = 32;   // TMEM columns: two buffers, a power of two
   while (columns < 2 * p.tn) columns <<= 1;
 
+  // the loading lane's place: tile, step, stage
+  int64_t lt = t0;
+  int lk = k0, ls = 0, lm = 0, ln = 0, loaded = 0;
+  uint32_t lphase = 0;
+  bool lok = true;
+  auto load_steps = [&]() {
+    while (lt < total && lok) {
+      if (lk == k0) tile_at(p, lt, lm, ln);
+      if (!mbar_wait(&sh.empty[ls], lphase ^ 1u, &sh.dead)) {
+        lok = false;
+        break;
+      }
+      uint8_t* dst = ring + ls * stage_bytes;
+      if (PAIR) {
+        const uint32_t bar = in_block(&sh.full[ls], 0);
+        if (rank == 0) mbar_expect(&sh.full[ls], 2 * stage_bytes);
+        tma_load_pair(dst, &map_b, lk * kMmaK, first_row_of(ln), bar);
+        tma_load_pair(dst + kMmaRows * kMmaK, &map_a, lk * kMmaK, lm * p.tn + rank * (rows_of(lm) / 2), bar);
+      } else {
+        mbar_expect(&sh.full[ls], stage_bytes);
+        tma_load(dst, &map_b, lk * kMmaK, first_row_of(ln), &sh.full[ls]);
+        tma_load(dst + kMmaRows * kMmaK, &map_a, lk * kMmaK, lm * p.tn, &sh.full[ls]);
+      }
+      loaded = min(loaded + 1, p.stages);
+      if (++ls == p.stages) {
+        ls = 0;
+        lphase ^= 1u;
+      }
+      if (++lk == k1) {
+        lk = k0;
+        lt += dt;
+      }
+    }
+  };
   if (warp == 0) {
     if (lane == 0) {
       for (int i = 0; i < p.stages; ++i) {
@@ -597,43 +631,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) mma_kernel(const __grid_consta
 
   if (warp == 0) {
     if (lane == 0) {
-      int s = 0, issued = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int64_t t = t0; t < total && ok; t += dt) {
-        int im, in;
-        tile_at(p, t, im, in);
-        for (int kb = k0; kb < k1; ++kb) {
-          if (!mbar_wait(&sh.empty[s], phase ^ 1u, &sh.dead)) {
-            ok = false;
-            break;
-          }
-          uint8_t* dst = ring + s * stage_bytes;
-          if (PAIR) {
-            const uint32_t bar = in_block(&sh.full[s], 0);
-            if (rank == 0) mbar_expect(&sh.full[s], 2 * stage_bytes);
-            tma_load_pair(dst, &map_b, kb * kMmaK, first_row_of(in), bar);
-            tma_load_pair(dst + kMmaRows * kMmaK, &map_a, kb * kMmaK, im * p.tn + rank * (rows_of(im) / 2), bar);
-          } else {
-            mbar_expect(&sh.full[s], stage_bytes);
-            tma_load(dst, &map_b, kb * kMmaK, first_row_of(in), &sh.full[s]);
-            tma_load(dst + kMmaRows * kMmaK, &map_a, kb * kMmaK, im * p.tn, &sh.full[s]);
-          }
-          issued = min(issued + 1, p.stages);
-          if (++s == p.stages) {
-            s = 0;
-            phase ^= 1u;
-          }
-        }
-      }
+      load_steps();
       // on giving up, copies may still be in flight: see each stage's last one
       // through (a stage whose copy was consumed long ago has passed its phase);
       // a pair's are counted by the first block, and the other ends after it
-      if (!ok && !(PAIR && rank))
-        for (int i = 0; i < issued; ++i) {
-          const int st = (s - 1 - i + 2 * p.stages) % p.stages;
-          const uint32_t ph = st < s ? phase : phase ^ 1u;
-          mbar_drain(&sh.full[st], ph);
+      if (!lok && !(PAIR && rank))
+        for (int i = 0; i < loaded; ++i) {
+          const int st = (ls - 1 - i + 2 * p.stages) % p.stages;
+          mbar_drain(&sh.full[st], st < ls ? lphase : lphase ^ 1u);
         }
     }
   } else if (warp == 1) {
@@ -959,6 +964,10 @@ cudaError_t launch_matmul_i8(const int8_t* a, int64_t m, int64_t as, const float
   auto run = [&](auto fn) -> cudaError_t {
     cudaError_t r = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (r != cudaSuccess) return r;
+    if (cluster == 1) {
+      fn<<<static_cast<unsigned>(blocks), kMmaThreads, smem, st>>>(ma, mb, p);
+      return cudaGetLastError();
+    }
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = static_cast<unsigned>(cluster);
