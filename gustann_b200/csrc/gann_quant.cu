@@ -906,8 +906,11 @@ struct MmaPlan {
 
 // Rows of a in a tile: all of them up to 256, in steps that the two output
 // halves share; with more, 256, halved while the tiles do not fill the GPU.
-// A tile's k is split over 2, 4 or 8 blocks while blocks are idle and each
-// part keeps four steps of 128. Full-width tiles are made by pairs.
+// A tile's k is split over 2, 4 or 8 blocks while blocks are idle, if that
+// saves more than it costs: a step of 128 takes a lone block about 0.36 us, the
+// exchange of the parts' sums 2.8 us and 0.05 us a column (16 x 4096 x 4096:
+// 12.9 us in two parts, 10.5 in four; 64 x 8192 x 1024: 11.6 in two, 7.1 in
+// one). Full-width tiles are made by pairs.
 MmaPlan plan_mma(int64_t m, int64_t n, int k, int sm_count) {
   MmaPlan p{16, 1, false};
   while (p.tn < m && p.tn < kMmaMaxTn) p.tn <<= 1;
@@ -915,7 +918,8 @@ MmaPlan plan_mma(int64_t m, int64_t n, int k, int sm_count) {
   while (m > p.tn / 2 && p.tn > 64 && tn_tiles * ((m + p.tn - 1) / p.tn) * 2 <= sm_count) p.tn >>= 1;
   const int64_t tiles = tn_tiles * ((m + p.tn - 1) / p.tn);
   const int steps = (k + kMmaK - 1) / kMmaK;
-  while (p.split < 8 && tiles * p.split * 2 <= sm_count && steps >= p.split * 8) p.split <<= 1;
+  while (p.split < 8 && tiles * p.split * 2 <= sm_count && steps >= p.split * 4) p.split <<= 1;
+  if (steps * (p.split - 1) * 36 < (280 + 5 * p.tn) * p.split) p.split = 1;
   p.pair = p.tn == kMmaMaxTn && p.split == 1 && n > kMmaRows;
   return p;
 }
