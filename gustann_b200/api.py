@@ -513,7 +513,9 @@ def quantize_rows(x, stream: int | None = None):
     int8 [n, d], scales float32 [n])``; the codes' rows start on 16-byte
     boundaries, as :func:`matmul_i8` wants them. A row with a NaN or an
     infinity gets scale NaN and codes 0. ``stream``: a ``cudaStream_t``, or
-    None for torch's current stream."""
+    None for torch's current stream; tensors made on other streams must stay
+    alive until it has passed the call. No gradients are recorded, here and in
+    the three calls below."""
     torch = _get_torch()
     if x.dim() != 2:
         _fail("quantize_rows: x must have two dimensions")

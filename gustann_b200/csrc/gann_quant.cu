@@ -959,7 +959,11 @@ cudaError_t launch_matmul_i8(const int8_t* a, int64_t m, int64_t as, const float
   p.stages = std::min({kMmaMaxStages, (200 * 1024) / stage, std::max(2, (k + kMmaK - 1) / kMmaK * 2)});
   const size_t ring = std::max<size_t>(static_cast<size_t>(p.stages) * stage,
                                        p.split > 1 ? static_cast<size_t>(p.tn) * kMmaRows * 4 : 0);
-  const size_t smem = ring + 1024;
+  // The blocks of a cluster all need their TMEM at once: two clusters on the
+  // same two SMs, each holding one SM's TMEM and waiting for the other's, would
+  // wait for ever. More than half of an SM's shared memory keeps a second one
+  // away, whatever runs on other streams.
+  const size_t smem = std::max<size_t>(ring + 1024, cluster > 1 ? 120 * 1024 : 0);
   CUtensorMap ma, mb;
   cudaError_t e = encode_rows(&ma, a, m, as, k, a_rows);
   if (e == cudaSuccess) e = encode_rows(&mb, b, n, bs, k, kMmaRows);

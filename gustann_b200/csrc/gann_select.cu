@@ -878,12 +878,13 @@ __global__ void __launch_bounds__(256) reorder_kernel(const __grid_constant__ St
 namespace {
 
 // How a call is run. Without softmax a warp can take a whole group: one
-// launch, nothing written but the result. That needs enough groups to fill the
-// GPU, or groups so small that one warp is done at once. Everything else is
-// split: rows into segments, a warp each, as many as the GPU holds at a time,
-// and joined by a second kernel.
+// launch, nothing written but the result. That wants groups so small that a
+// lone warp is done at once, or enough of them to fill the GPU and none so
+// large that a warp's one tile at a time cannot keep the memory busy.
+// Everything else is split: rows into segments, a warp each, as many as the
+// GPU holds at a time, and joined by a second kernel.
 constexpr int kResidentWarps = 148 * 20;
-constexpr int kSmallGroup = 4096;      // bytes of a group that a lone warp reads in one tile
+constexpr int kSmallGroup = 4096, kLargeGroup = 65536;   // bytes of a group
 
 struct SelectPlan {
   bool split = false;
@@ -894,7 +895,7 @@ SelectPlan plan_select(int64_t groups, int beams, int vocab, int dtype, bool sof
   SelectPlan p;
   const int elem = dtype == GANN_F32 ? 4 : 2, n = 16 / elem;
   const int64_t bytes = static_cast<int64_t>(beams) * vocab * elem;
-  p.split = softmax || !(bytes <= kSmallGroup || groups >= kResidentWarps / 4);
+  p.split = softmax || !(bytes <= kSmallGroup || (bytes <= kLargeGroup && groups >= kResidentWarps / 4));
   if (!p.split) return p;
   const int64_t rows = std::max<int64_t>(1, groups * beams);
   const int64_t tiles = (static_cast<int64_t>(vocab) + n - 1 + kRowTile * n - 1) / (kRowTile * n);   // a row may start inside a vector

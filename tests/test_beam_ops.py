@@ -99,7 +99,8 @@ def make(g, w, v, dtype, seed, spread=3.0):
 SIZES = [(1, 1, 1, 1), (1, 1, 5, 9), (1, 4, 32001, 8), (3, 2, 17, 4), (2, 4, 4099, 8), (2, 1, 50000, 1),
          (1, 3, 131075, 32), (5, 8, 256, 8), (40, 32, 16, 32), (300, 8, 100, 100), (7, 64, 10, 128), (2, 128, 33, 128),
          (1, 128, 3000, 128), (2, 16, 9000, 33), (1, 2, 70001, 128), (1000, 4, 64, 16), (9, 5, 1023, 64),
-         (33, 1, 2048, 2), (3, 7, 8191, 17), (4, 2, 20000, 65)]
+         (33, 1, 2048, 2), (3, 7, 8191, 17), (4, 2, 20000, 65), (800, 2, 4000, 8), (800, 2, 9000, 24),
+         (760, 3, 700, 90)]
 
 
 @pytest.mark.gpu

@@ -199,6 +199,25 @@ def test_output_offsets_past_32_bits():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(1024, 20000, 64), (600, 30000, 200), (16, 600, 4096), (200, 300, 8192)])
+def test_calls_at_the_same_time(m, n, k):
+    """Large products with a short k, and split ones, on four streams at once:
+    blocks that work in clusters do not wait for each other's SMs."""
+    a, sa = i8(m, k, 1)
+    b, sb = i8(n, k, 2)
+    want = matmul_i8(a, sa, b, sb, dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    outs = []
+    for _ in range(6):
+        for st in streams:
+            with torch.cuda.stream(st):
+                outs.append(matmul_i8(a, sa, b, sb, dtype=torch.bfloat16))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.gpu
 def test_streams_and_graphs():
     x = torch.randn(50, 200, device="cuda")
     b, sb = quantize_rows(torch.randn(300, 200, device="cuda"))
