@@ -264,6 +264,9 @@ struct Held {
 //     compared with the least kept key and listed, one a lane at a time. The
 //     list is sorted and cut when it is full, which raises the threshold.
 // A segment writes its `keep` best and its sum; merge_kernel joins them.
+// Bound by instructions: 64 x 4 x 128000 bf16 with log-softmax takes 34 us with
+// its join (1.9 TB/s; reading alone would be 10), about 14 warp instructions an
+// element, of which the exponential, its argument and sum are four.
 constexpr int kRowWarps = 4, kRowVecs = 4;
 constexpr int kRowTile = kRowVecs * kWarp;   // vectors
 
@@ -272,7 +275,7 @@ struct SegStat {
 };
 
 template <typename T, bool SOFTMAX, bool LONG>
-__global__ void __launch_bounds__(kRowWarps* kWarp, 5) row_kernel(const T* __restrict__ logits, int64_t gstride,
+__global__ void __launch_bounds__(kRowWarps* kWarp, 4) row_kernel(const T* __restrict__ logits, int64_t gstride,
                                                                int64_t bstride, const float* __restrict__ scores,
                                                                const uint8_t* __restrict__ finished, int64_t rows,
                                                                int beams, int vocab, int keep, int segs, int seg_tiles,
@@ -451,6 +454,9 @@ __global__ void __launch_bounds__(kRowWarps* kWarp, 5) row_kernel(const T* __res
 // passes are read again (from L1), one a lane at a time, and their elements at
 // or above the threshold are listed as (f, index); the sort by that is looked
 // over for equal f, which are put in the order of their 64-bit values.
+// 100000 x 8 x 256 f32, keep 8: 182 us (4.6 TB/s), bound by instructions and
+// the latency of one tile a warp; 10000 x 8 x 100, keep 100: 52 us, most of it
+// the sort of 128.
 constexpr int kGroupWarps = 4;
 
 template <typename T, int VW>
@@ -693,14 +699,17 @@ __global__ void __launch_bounds__(kGroupWarps* kWarp, NV * VW > 32 ? 5 : 7) grou
 // keeps its best in a sorted list; a candidate's place in the result is its
 // place in its own list plus, for every other list, the number of keys above
 // it (binary search).
-constexpr int kMergeWarps = 8;
+template <bool LONG>
+struct Merge {
+  static constexpr int warps = LONG ? 8 : 16;
+};
 
 template <bool LONG>
-__global__ void __launch_bounds__(kMergeWarps* kWarp) merge_kernel(
+__global__ void __launch_bounds__(Merge<LONG>::warps* kWarp) merge_kernel(
     const Key1* __restrict__ cand, const SegStat* __restrict__ stats, const float* __restrict__ scores,
     const uint8_t* __restrict__ finished, int64_t groups, int beams, int vocab, int keep, int segs, int softmax,
     int end_token, float* __restrict__ out_s, int32_t* __restrict__ out_p, int32_t* __restrict__ out_t) {
-  constexpr int kCap = Held<LONG>::value;
+  constexpr int kCap = Held<LONG>::value, kMergeWarps = Merge<LONG>::warps;
   __shared__ double offs[kBeamMax], tops[kBeamMax];   // v = offs + (x - tops)
   __shared__ uint8_t kind[kBeamMax];                  // 0 no candidates, 1 lists, 2 finished
   __shared__ Key2 lists[kMergeWarps][kCap];
@@ -821,7 +830,8 @@ struct StateTable {
 // writes any, so source and target may be the same rows; rows that stay where
 // they are are not touched. MAX 0: source and target are apart, and eight rows
 // at a time are on their way. Bound by memory: each kept row is written once
-// and each distinct parent read once from DRAM (again from the caches).
+// and each distinct parent read once from DRAM (again from the caches); four
+// caches of 16 x 4 beams, 0.9 GB, take 141 us (6.4 TB/s).
 template <typename U, int MAX>
 __global__ void __launch_bounds__(256) reorder_kernel(const __grid_constant__ StateTable tab,
                                                       const int32_t* __restrict__ parents, int beams, int keep) {
@@ -882,8 +892,11 @@ namespace {
 // lone warp is done at once, or enough of them to fill the GPU and none so
 // large that a warp's one tile at a time cannot keep the memory busy.
 // Everything else is split: rows into segments, a warp each, as many as the
-// GPU holds at a time, and joined by a second kernel.
-constexpr int kResidentWarps = 148 * 20;
+// GPU holds at a time, and joined by a second kernel. Sixteen warps an SM: more
+// warps leave each fewer tiles to pay for its threshold with and the join more
+// candidates (64 x 4 x 128000 bf16, keep 8: 34 us with 16, 35 with 20, 38 with
+// 24, 45 with 32).
+constexpr int kResidentWarps = 148 * 16;
 constexpr int kSmallGroup = 4096, kLargeGroup = 65536;   // bytes of a group
 
 struct SelectPlan {
@@ -900,7 +913,8 @@ SelectPlan plan_select(int64_t groups, int beams, int vocab, int dtype, bool sof
   const int64_t rows = std::max<int64_t>(1, groups * beams);
   const int64_t tiles = (static_cast<int64_t>(vocab) + n - 1 + kRowTile * n - 1) / (kRowTile * n);   // a row may start inside a vector
   const int64_t want = std::max<int64_t>(1, kResidentWarps / rows);
-  p.seg_tiles = static_cast<int>((tiles + want - 1) / want);
+  // at least four tiles a warp, or the join has more to do than is saved
+  p.seg_tiles = static_cast<int>(std::min<int64_t>(tiles, std::max<int64_t>(4, (tiles + want - 1) / want)));
   p.segs = static_cast<int>((tiles + p.seg_tiles - 1) / p.seg_tiles);
   return p;
 }
@@ -969,7 +983,7 @@ cudaError_t run_split(const SelectArgs& a, const SelectPlan& p, int sm_count, cu
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(a.groups, static_cast<int64_t>(sm_count) * 64)));
-  cfg.blockDim = dim3(kMergeWarps * kWarp);
+  cfg.blockDim = dim3((many ? Merge<true>::warps : Merge<false>::warps) * kWarp);
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
