@@ -374,6 +374,7 @@ __global__ void __launch_bounds__(kRowWarps* kWarp, 4) row_kernel(const T* __res
         }
         thr = unord32(lo);
       }
+      thr = fmaxf(thr, -3.402823466e+38f);   // masked elements are below every float
     }
     const int64_t p0 = first + static_cast<int64_t>(t) * kRowTile * N;
     if (__any_sync(kFull, mx >= thr)) {
