@@ -173,6 +173,10 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 constexpr float kLog2e = 1.4426950408889634f;
+// Row maxima of less than 2^17 have x log2e rounded by at most 2^-7, whose e^-d
+// is 1 - d + d^2 / 2 to 3e-8. With larger ones the terms are exp(x - maximum),
+// an instruction more each.
+constexpr float kFarMax = 131072.f;
 
 __device__ __forceinline__ bool live(float score) { return fabsf(score) < INFINITY; }
 
@@ -406,18 +410,19 @@ __global__ void __launch_bounds__(kRowWarps* kWarp, 4) row_kernel(const T* __res
         sum *= static_cast<double>(fast_exp2((m - mx) * kLog2e));
         m = mx;
         m2 = m * kLog2e;
-        fix = 1.f - __fmaf_rn(m, kLog2e, -m2) * 0.6931471805599453f;
+        const float d = __fmaf_rn(m, kLog2e, -m2) * 0.6931471805599453f;
+        fix = fabsf(m) < kFarMax ? __fmaf_rn(d, __fmaf_rn(0.5f, d, -1.f), 1.f) : kNan;
       }
       float part = 0.f;
       if (m > -INFINITY) {
-        // 2^(x log2e - m2), one fused step an element; `fix` makes up for m2's
-        // rounding
+        // 2^(x log2e - m2), one fused step an element; `fix` = e^-d makes up
+        // for m2's rounding d
 #pragma unroll
         for (int i = 0; i < kRowVecs; ++i)
 #pragma unroll
           for (int j = 0; j < N; ++j) part += fast_exp2(__fmaf_rn(Raw<T>::at(cur[i], j), kLog2e, -m2));
         part *= fix;
-        if (!(part >= 0.f && part < INFINITY)) {   // a NaN or infinite entry, or m2 past float32: again without
+        if (!(part >= 0.f && part < INFINITY)) {   // a NaN or infinite entry, or a maximum far from 0: again without
           part = 0.f;
 #pragma unroll
           for (int i = 0; i < kRowVecs; ++i)

@@ -198,6 +198,26 @@ def test_select_strides_and_alignment(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,offset", [(d, o) for d, offs in (
+    ("f32", (1e4, -65504.0, 1e5, -1.31e5, 1.32e5, -1e6, 1e7, 3e7, -5e7, 1e8, -1e9, 1e10, -1e12, 1e30, -3e38)),
+    ("f16", (1e4, 65504.0, -65504.0)), ("bf16", (1e4, -1e5, 1e6, 3e7, -1e9, 1e12, -1e30))) for o in offs])
+def test_log_softmax_of_rows_far_from_zero(dtype, offset):
+    """A constant added to a row changes no candidate's value: rows around the
+    offset, one row of the offset alone (every token masked by a large finite
+    number) beside ordinary ones, and a row with a few tokens left. The terms
+    are taken relative to the maximum, so the derivation of LSE holds as it is."""
+    for g, w, v, k in ((2, 4, 3001, 8), (1, 3, 20000, 40)):
+        sc, lg = make(g, w, v, dtype, 11)
+        check_select(sc, (lg.float() + offset).clamp(torch.finfo(lg.dtype).min, torch.finfo(lg.dtype).max).to(lg.dtype),
+                     k, True)
+        one = lg.clone()
+        one[:, 1] = offset
+        check_select(sc, one, k, True)
+        one[:, 2, 5:] = offset
+        check_select(sc, one, k, True)
+
+
+@pytest.mark.gpu
 def test_select_offsets_past_32_bits():
     """A group stride that puts the last group 2^31 elements behind the first."""
     lg = torch.zeros(2 ** 31 + 4096, dtype=torch.float16, device="cuda").as_strided((2, 2, 1000), (2 ** 31, 1000, 1))
