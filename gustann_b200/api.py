@@ -608,8 +608,10 @@ def beam_select(scores, logits, k: int, log_softmax: bool = False, finished=None
     ``scores`` [g, w] float32, ``logits`` [g, w, v] float32, float16 or bfloat16
     (any strides with v contiguous). A candidate is worth ``scores[g, b] +
     logits[g, b, t]``, or with ``log_softmax`` ``scores[g, b] +
-    log_softmax(logits[g, b])[t]``; the largest come first, equal ones in
-    ascending order of (b, t). Logits that are NaN or infinite are masked;
+    log_softmax(logits[g, b])[t]``; the largest come first, compared in 64 bits,
+    equal ones in ascending order of (b, t) (with ``log_softmax`` a beam's own
+    candidates by ``scores + logits``, then t; those of different beams may trade
+    places where their values are within 2^-17). Logits that are NaN or infinite are masked;
     beams whose score is not finite are dead. ``finished`` [g, w] bool: such a
     beam has one candidate, ``end_token`` at its own score. Returns ``(scores
     float32, parents int32, tokens int32)``, each [g, k], filled up with

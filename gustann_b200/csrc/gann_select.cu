@@ -3,8 +3,9 @@
 // The candidate (b, t) of a group is worth
 //   v = S_b + L_bt                      or, with log-softmax,
 //   v = S_b + (L_bt - max_t L_bt) - log(sum_t exp(L_bt - max_t L_bt)),
-// compared in 64 bits; equal values go to the lower b * V + t. Entries that
-// are not finite are no candidates, neither are those of a beam whose S is
+// compared in 64 bits; equal values go to the lower b * V + t. With log-softmax
+// a beam's own candidates are ordered by S_b + L_bt in 64 bits, then t. Entries
+// that are not finite are no candidates, neither are those of a beam whose S is
 // not finite. A finished beam offers (b, end_token) alone, worth S_b.
 #include <algorithm>
 #include <cmath>
@@ -106,21 +107,59 @@ __device__ __forceinline__ double unord64(uint64_t b) {
 }
 
 // Sort keys, largest first. Key1: a float's order and the complement of an
-// index in one word; Key2: a double's order, then the complement of an index.
-// The all-zero key stands behind every candidate.
+// index in one word; Key2: a double's order, then (see Place) what settles
+// equal ones. The all-zero key stands behind every candidate.
 struct Key1 {
   uint64_t a;
   __device__ bool above(const Key1& o) const { return a > o.a; }
   __device__ Key1 from(int lane_mask) const { return {__shfl_xor_sync(kFull, a, lane_mask)}; }
 };
 struct Key2 {
-  uint64_t a;
-  uint32_t b;
+  uint64_t a, b;
   __device__ bool above(const Key2& o) const { return a > o.a || (a == o.a && b > o.b); }
   __device__ Key2 from(int lane_mask) const {
     return {__shfl_xor_sync(kFull, a, lane_mask), __shfl_xor_sync(kFull, b, lane_mask)};
   }
 };
+
+// Equal values: the lower beam first, within a beam the larger x (log-softmax
+// can round the values of two x to one), then the lower token, packed so that
+// the larger word comes first. beams * vocab < 2^31 leaves both numbers 32 bits.
+struct Place {
+  int token_bits;
+  uint32_t last_beam;
+  __device__ static Place of(int beams, int vocab) {
+    return {32 - __clz(vocab - 1), static_cast<uint32_t>(beams) - 1};
+  }
+  __device__ uint64_t pack(uint32_t b, uint32_t x, uint32_t t) const {
+    const uint64_t low = (static_cast<uint64_t>(1) << token_bits) - 1;
+    return static_cast<uint64_t>(last_beam - b) << (32 + token_bits) | static_cast<uint64_t>(x) << token_bits | (low - t);
+  }
+  __device__ uint32_t beam(uint64_t p) const { return last_beam - static_cast<uint32_t>(p >> (32 + token_bits)); }
+  __device__ uint32_t token(uint64_t p) const {
+    const uint64_t low = (static_cast<uint64_t>(1) << token_bits) - 1;
+    return static_cast<uint32_t>(low - (p & low));
+  }
+};
+
+// One x for all that have the same sum with s in 64 bits: the sum less s. That
+// is x itself unless s is so large that the sum rounds x to fewer bits, and
+// float32 holds it either way (|x| >= |s|: off by 2^-52 of x, which rounds back;
+// |x| < |s|: the difference is exact, a rounding of x). From |x| = 2^-27 |s| on
+// the sum's step is at most x's and the sum exact.
+// A call, not inlined: rows whose every element passes the threshold run the loop
+// around it 16 to 32 times a tile (64 x 4 x 128000 equal bf16: rows 110 us
+// without it, 118 with the call, 121 inlined).
+__device__ __noinline__ float same_sum(float x, float s) {
+  const double d = static_cast<double>(s);
+  return static_cast<float>((d + static_cast<double>(x)) - d);
+}
+// A float that is not above any x with the same sum: those are within one step
+// of the sum, which is at most 2^-52 of it.
+__device__ __forceinline__ float below_same_sum(float x, float s) {
+  const double d = static_cast<double>(x);
+  return __double2float_rd(d - fabs(static_cast<double>(s) + d) * 0x1p-52);
+}
 
 // Whether a lane keeps the larger key at a step of a bitonic sort (largest
 // first) over lanes: bit log2(size) of the lane equals bit log2(stride).
@@ -267,6 +306,8 @@ struct Held {
 //     mark their elements at or above the threshold; the marked ones are
 //     compared with the least kept key and listed, one a lane at a time. The
 //     list is sorted and cut when it is full, which raises the threshold.
+//     Listed is same_sum(x), so that the order is that of the 64-bit sums with
+//     the score; the threshold lies at or below every x of an equal sum.
 // A segment writes its `keep` best and its sum; merge_kernel joins them.
 // Bound by instructions: 64 x 4 x 128000 bf16 with log-softmax takes 34 us with
 // its join (1.9 TB/s; reading alone would be 10), about 14 warp instructions an
@@ -293,7 +334,8 @@ __global__ void __launch_bounds__(kRowWarps* kWarp, 4) row_kernel(const T* __res
   if (item >= rows * segs) return;
   const int64_t rw = item / segs;
   const int seg = static_cast<int>(item - rw * segs);
-  if (!live(scores[rw]) || (finished && finished[rw])) return;
+  const float score = scores[rw];
+  if (!live(score) || (finished && finished[rw])) return;
   const int64_t g = rw / beams;
   const T* row = logits + g * gstride + (rw - g * beams) * bstride;
   const int head = static_cast<int>((reinterpret_cast<uintptr_t>(row) % 16) / sizeof(T));
@@ -333,7 +375,7 @@ __global__ void __launch_bounds__(kRowWarps* kWarp, 4) row_kernel(const T* __res
     cnt = min(cnt, keep);
     if (cnt < keep) return;
     floor = list[keep - 1];
-    thr = unord32(static_cast<uint32_t>(floor.a >> 32));
+    thr = fmaxf(below_same_sum(unord32(static_cast<uint32_t>(floor.a >> 32)), score), -3.402823466e+38f);
   };
   double sum = 0.0;
   const int64_t last = (vocab - first + static_cast<int64_t>(kRowTile) * N - 1) / (static_cast<int64_t>(kRowTile) * N);
@@ -378,7 +420,7 @@ __global__ void __launch_bounds__(kRowWarps* kWarp, 4) row_kernel(const T* __res
         }
         thr = unord32(lo);
       }
-      thr = fmaxf(thr, -3.402823466e+38f);   // masked elements are below every float
+      thr = fmaxf(below_same_sum(thr, score), -3.402823466e+38f);   // masked elements are below every float
     }
     const int64_t p0 = first + static_cast<int64_t>(t) * kRowTile * N;
     if (__any_sync(kFull, mx >= thr)) {
@@ -390,11 +432,13 @@ __global__ void __launch_bounds__(kRowWarps* kWarp, 4) row_kernel(const T* __res
           for (int j = 0; j < N; ++j)
             if (Raw<T>::at(cur[i], j) >= thr) mark |= 1u << (i * N + j);
         }
+      const bool exact = thr >= fabsf(score) * 0x1p-27f || score == 0.f;   // same_sum(x) = x from thr on
       while (__any_sync(kFull, mark)) {
         if (cnt > kCap - kWarp) cut();
         const int e = __ffs(mark) - 1;
         const int64_t p = p0 + ((e / N) * kWarp + lane) * N + e % N;
-        const float x = mark && p >= 0 && p < vocab ? Raw<T>::one(row + p) : kNan;
+        float x = mark && p >= 0 && p < vocab ? Raw<T>::one(row + p) : kNan;
+        if (!exact) x = same_sum(x, score);
         const Key1 k{(static_cast<uint64_t>(ord32(x)) << 32) | ~static_cast<uint32_t>(p)};
         const bool take = fabsf(x) < INFINITY && k.above(floor);
         const unsigned pass = __ballot_sync(kFull, take);
@@ -721,6 +765,7 @@ __global__ void __launch_bounds__(Merge<LONG>::warps* kWarp) merge_kernel(
   __shared__ Key2 lists[kMergeWarps][kCap];
   __shared__ int counts[kMergeWarps];
   const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
+  const Place place = Place::of(beams, vocab);
   cudaGridDependencySynchronize();
   const int64_t per_beam = static_cast<int64_t>(segs) * keep, total = per_beam * beams;
   const bool small = total < (int64_t(1) << 31);
@@ -774,16 +819,17 @@ __global__ void __launch_bounds__(Merge<LONG>::warps* kWarp) merge_kernel(
           if (kind[b] == 1) {   // rows without candidates have no lists
             const uint64_t x = cand[g * total + at].a;
             take = x != 0;
+            const uint32_t o = static_cast<uint32_t>(x >> 32);
             if (take)
-              k = {ord64(offs[b] + (static_cast<double>(unord32(static_cast<uint32_t>(x >> 32))) - tops[b])),
-                   ~(static_cast<uint32_t>(b) * vocab + ~static_cast<uint32_t>(x))};
+              k = {ord64(offs[b] + (static_cast<double>(unord32(o)) - tops[b])),
+                   place.pack(b, o, ~static_cast<uint32_t>(x))};
           }
         }
         e += kWarp;
       } else {
         const int b = b0 + lane;
         take = b < beams && kind[b] == 2;
-        if (take) k = {ord64(static_cast<double>(sc[b])), ~(static_cast<uint32_t>(b) * vocab + end_token)};
+        if (take) k = {ord64(static_cast<double>(sc[b])), place.pack(b, 0, end_token)};
         b0 += kWarp;
       }
       take = take && k.above(floor);
@@ -812,10 +858,9 @@ __global__ void __launch_bounds__(Merge<LONG>::warps* kWarp) merge_kernel(
         rank += lo;
       }
       if (rank < keep) {
-        const uint32_t idx = ~k.b, b = idx / static_cast<uint32_t>(vocab);
         out_s[g * keep + rank] = static_cast<float>(unord64(k.a));
-        out_p[g * keep + rank] = static_cast<int32_t>(b);
-        out_t[g * keep + rank] = static_cast<int32_t>(idx - b * vocab);
+        out_p[g * keep + rank] = static_cast<int32_t>(place.beam(k.b));
+        out_t[g * keep + rank] = static_cast<int32_t>(place.token(k.b));
       }
     }
     for (int j = found + tid; j < keep; j += kMergeWarps * kWarp) {

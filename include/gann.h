@@ -404,8 +404,12 @@ int gann_matmul_i8(const int8_t* d_a, int64_t m, int64_t a_stride, const float* 
  *   scores[g][b] + logits[g][b][t]                                (log_softmax 0)
  *   scores[g][b] + logits[g][b][t] - log sum_t exp logits[g][b][t]            (1)
  * and the candidates are ordered by that value, largest first, compared in 64
- * bits, equal ones by b * vocab + t. (Pass negated distances.) The sum of the
- * exponentials is gathered in float32 and joined in 64 bits.
+ * bits, equal ones by b * vocab + t. (Pass negated distances.) With log_softmax
+ * the sum of the exponentials is gathered in float32 and joined in 64 bits, so
+ * the values of one beam share an error of less than 2^-17 (about 1e-7 as a
+ * rule), and candidates of different beams nearer than that to each other may
+ * trade places; a beam's own candidates are ordered by scores + logits in 64
+ * bits, equal ones by t.
  *   logits    [groups][beams][vocab] of dtype (gann_float); strides in elements
  *             (>= 0; 0 repeats a row), vocab contiguous. NaN and infinite entries are masked:
  *             no candidates, and not in the sum.

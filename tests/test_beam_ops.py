@@ -184,6 +184,56 @@ def test_values_closer_than_float32():
     check_select(sc, lg, 10)
 
 
+def equal_sums(g, w, v, dtype, score, kind):
+    """Scores so large beside the logits (or logits so small beside the scores)
+    that many different logits have one sum in 64 bits."""
+    sc, lg = make(g, w, v, dtype, v)
+    if kind == "tiny":
+        gen = torch.Generator(device="cuda").manual_seed(v)
+        lg = (1e-17 * torch.randint(-40, 41, lg.shape, generator=gen, device="cuda")).to(lg.dtype)
+    if kind == "one ordinary beam":
+        lg[:, 0, 5:] = float("-inf")      # too few to fill the result
+    sc = sc + score if kind == "spread" else torch.full_like(sc, score)
+    if kind == "one ordinary beam":
+        sc[:, 0] = -1.5
+    return sc, lg
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("score", [-5.0, -1e9, 1e12, -1e15, -3.4e38])
+@pytest.mark.parametrize("g,w,v,k", [(1, 2, 300, 9), (2, 3, 20011, 8), (1, 2, 40000, 128), (2, 4, 6000, 20)])
+def test_equal_sums_of_different_logits(g, w, v, k, score, dtype):
+    """Values are compared in 64 bits, whichever way the sizes are run."""
+    for kind in ("same", "spread", "tiny", "one ordinary beam"):
+        check_select(*equal_sums(g, w, v, dtype, score, kind), k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("score", [-5.0, -1e9, 1e12, -1e15, -3.4e38])
+@pytest.mark.parametrize("g,w,v,k", [(1, 2, 300, 9), (2, 3, 20011, 8), (1, 2, 40000, 128)])
+def test_equal_sums_with_log_softmax(g, w, v, k, score, dtype):
+    """A beam's own candidates come by score + logit in 64 bits, then token. The
+    value is rounded three times in 64 bits beside the logarithm's error, each
+    time by half a step of at most 2^-52 of the score (other terms: LSE)."""
+    for kind in ("same", "spread", "tiny", "one ordinary beam"):
+        sc, lg = equal_sums(g, w, v, dtype, score, kind)
+        s, p, t = (x.cpu().numpy() for x in beam_select(sc, lg, k, log_softmax=True))
+        values = ref_values(sc, lg, True)
+        rv, rp, _ = ref_select(sc, lg, k, True, values=values)
+        assert np.array_equal(p < 0, rp < 0)
+        sums = sc.cpu().double().numpy()[:, :, None] + lg.cpu().double().numpy()
+        off = 2 * (LSE + 4 * 2.0 ** -53 * abs(score))
+        for i in range(g):
+            n = int((p[i] >= 0).sum())
+            assert bool((np.abs(values[i, p[i, :n] * v + t[i, :n]] - rv[i, :n]) <= off).all())
+            assert bool((np.abs(s[i, :n] - rv[i, :n]) <= off + 1.01 * 2.0 ** -24 * np.abs(rv[i, :n])).all())
+            for b in set(p[i, :n].tolist()):
+                f = t[i, :n][p[i, :n] == b]
+                assert np.array_equal(f, np.lexsort((np.arange(v), -sums[i, b]))[:f.size])
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(DT))
 def test_select_strides_and_alignment(dtype):
