@@ -968,13 +968,14 @@ cudaError_t launch_matmul_i8(const int8_t* a, int64_t m, int64_t as, const float
   // wait for ever. More than half of an SM's shared memory keeps a second one
   // away, whatever runs on other streams.
   const size_t smem = std::max<size_t>(ring + 1024, cluster > 1 ? 120 * 1024 : 0);
-  CUtensorMap ma, mb;
-  cudaError_t e = encode_rows(&ma, a, m, as, k, a_rows);
-  if (e == cudaSuccess) e = encode_rows(&mb, b, n, bs, k, kMmaRows);
-  if (e != cudaSuccess) return e;
   const int64_t blocks = cluster * (p.split > 1 ? tiles_m * tiles_n : std::min<int64_t>(tiles_m * tiles_n, sm_count / cluster));
   auto run = [&](auto fn) -> cudaError_t {
     cudaError_t r = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    // the driver's call wants a context, which the one before has made current
+    // if this is the host thread's first
+    CUtensorMap ma, mb;
+    if (r == cudaSuccess) r = encode_rows(&ma, a, m, as, k, a_rows);
+    if (r == cudaSuccess) r = encode_rows(&mb, b, n, bs, k, kMmaRows);
     if (r != cudaSuccess) return r;
     if (cluster == 1) {
       fn<<<static_cast<unsigned>(blocks), kMmaThreads, smem, st>>>(ma, mb, p);

@@ -1,6 +1,7 @@
 """8-bit rows (gann_quantize_rows) and their products (gann_matmul_i8) against
 exact arithmetic in 64 bits."""
 import ctypes as C
+import threading
 
 import numpy as np
 import pytest
@@ -215,6 +216,25 @@ def test_calls_at_the_same_time(m, n, k):
                 outs.append(matmul_i8(a, sa, b, sb, dtype=torch.bfloat16))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 40])
+def test_first_cuda_call_of_a_thread(m):
+    """A host thread that has made no CUDA call before calls the C entry."""
+    a, sa = i8(m, 64, 1)
+    b, sb = i8(70, 64, 2)
+    want = matmul_i8(a, sa, b, sb)
+    got = torch.zeros_like(want)
+    args = (a.data_ptr(), m, 64, sa.data_ptr(), b.data_ptr(), 70, 64, sb.data_ptr(), None, 64, got.data_ptr(), 70,
+            api.F32, 0, None)
+    torch.cuda.synchronize()
+    code = []
+    t = threading.Thread(target=lambda: code.append(api.lib.gann_matmul_i8(*args)))
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert code == [api.GANN_OK] and torch.equal(got, want)
 
 
 @pytest.mark.gpu
