@@ -352,6 +352,11 @@ struct MmaShared {
   __align__(16) float sa[2][kMmaMaxTn];
 };
 
+// The most dynamic shared memory that a block may ask for beside MmaShared, and
+// the kernels' limit: one value for every call, for a limit that followed the
+// call's own size could fall below another thread's before that one launches.
+constexpr size_t kMmaSmem = (227 * 1024 - sizeof(MmaShared)) / 128 * 128;
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void mbar_init(uint64_t* b, int n) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(n) : "memory");
@@ -970,7 +975,7 @@ cudaError_t launch_matmul_i8(const int8_t* a, int64_t m, int64_t as, const float
   const size_t smem = std::max<size_t>(ring + 1024, cluster > 1 ? 120 * 1024 : 0);
   const int64_t blocks = cluster * (p.split > 1 ? tiles_m * tiles_n : std::min<int64_t>(tiles_m * tiles_n, sm_count / cluster));
   auto run = [&](auto fn) -> cudaError_t {
-    cudaError_t r = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    cudaError_t r = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMmaSmem));
     // the driver's call wants a context, which the one before has made current
     // if this is the host thread's first
     CUtensorMap ma, mb;

@@ -238,6 +238,38 @@ def test_first_cuda_call_of_a_thread(m):
 
 
 @pytest.mark.gpu
+def test_products_of_different_sizes_from_several_threads():
+    """Plans with little and with much shared memory, launched by four threads
+    at once (the library is called without the interpreter's lock)."""
+    work = []
+    for m, n, k in ((16, 300, 33), (16, 600, 4096), (100, 3000, 512), (8, 200, 64)):
+        a, sa = i8(m, k, 1)
+        b, sb = i8(n, k, 2)
+        want = matmul_i8(a, sa, b, sb)
+        got = torch.empty_like(want)
+        args = (a.data_ptr(), m, a.stride(0), sa.data_ptr(), b.data_ptr(), n, b.stride(0), sb.data_ptr(), None, k,
+                got.data_ptr(), n, api.F32, 0, torch.cuda.Stream().cuda_stream)
+        work.append((args, got, want, a, sa, b, sb))
+    torch.cuda.synchronize()
+    start, errors = threading.Barrier(4), []
+
+    def run(args, *_):
+        start.wait()
+        for _ in range(5000):
+            if api.lib.gann_matmul_i8(*args):
+                errors.append(api.lib.gann_last_error())
+                return
+    threads = [threading.Thread(target=run, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert errors == []
+    assert all(torch.equal(w[1], w[2]) for w in work)
+
+
+@pytest.mark.gpu
 def test_streams_and_graphs():
     x = torch.randn(50, 200, device="cuda")
     b, sb = quantize_rows(torch.randn(300, 200, device="cuda"))
