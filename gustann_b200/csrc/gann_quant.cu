@@ -327,8 +327,15 @@ __global__ void __launch_bounds__(kThinThreads) thin_kernel(const int8_t* __rest
 // there), 4097 x 4096 x 4096 to bf16 58 us, 4096 x 131072 x 768 to f32 500 us
 // (the output alone is 330 us of writes), 24 x 32001 x 1024 12 us.
 //
-// Every wait ends: after kWaitClocks the block gives up, and the tiles it has not
-// finished are filled with NaN.
+// Waits for copies, products and buffers end: after kWaitClocks the block gives
+// up, and the tiles it has not finished are filled with NaN (there is no other
+// sign of it). The allocation of TMEM and the clusters' barriers have no limit of
+// their own. A lone block waits for TMEM while it holds none, so whoever has it
+// goes on and frees it. The blocks of a cluster need theirs all at once, and two
+// clusters on the same SMs could each hold what the other waits for: a block of a
+// cluster therefore asks for all of an SM's shared memory, which leaves no room
+// for any other block, of this kernel or another, until it ends. The barriers
+// wait only for the cluster's own blocks, each of which gets there.
 constexpr int kEpiWarps = 8, kEpiThreads = kEpiWarps * kWarp;
 constexpr int kMmaThreads = kEpiThreads + 2 * kWarp;
 constexpr int kMmaRows = 128, kMmaK = 128;
@@ -356,6 +363,8 @@ struct MmaShared {
 // the kernels' limit: one value for every call, for a limit that followed the
 // call's own size could fall below another thread's before that one launches.
 constexpr size_t kMmaSmem = (227 * 1024 - sizeof(MmaShared)) / 128 * 128;
+// With the 1 KB that every block is charged, an SM of 228 KB has less than that left.
+static_assert(228 * 1024 - 1024 - kMmaSmem - sizeof(MmaShared) < 1024, "another block would fit beside a cluster's");
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void mbar_init(uint64_t* b, int n) {
@@ -968,11 +977,8 @@ cudaError_t launch_matmul_i8(const int8_t* a, int64_t m, int64_t as, const float
   p.stages = std::min({kMmaMaxStages, (200 * 1024) / stage, std::max(2, (k + kMmaK - 1) / kMmaK * 2)});
   const size_t ring = std::max<size_t>(static_cast<size_t>(p.stages) * stage,
                                        p.split > 1 ? static_cast<size_t>(p.tn) * kMmaRows * 4 : 0);
-  // The blocks of a cluster all need their TMEM at once: two clusters on the
-  // same two SMs, each holding one SM's TMEM and waiting for the other's, would
-  // wait for ever. More than half of an SM's shared memory keeps a second one
-  // away, whatever runs on other streams.
-  const size_t smem = std::max<size_t>(ring + 1024, cluster > 1 ? 120 * 1024 : 0);
+  const size_t smem = cluster > 1 ? kMmaSmem : ring + 1024;   // a cluster's blocks have their SMs to themselves
+  if (ring + 1024 > kMmaSmem) return cudaErrorInvalidConfiguration;
   const int64_t blocks = cluster * (p.split > 1 ? tiles_m * tiles_n : std::min<int64_t>(tiles_m * tiles_n, sm_count / cluster));
   auto run = [&](auto fn) -> cudaError_t {
     cudaError_t r = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMmaSmem));

@@ -269,6 +269,55 @@ def test_products_of_different_sizes_from_several_threads():
     assert all(torch.equal(w[1], w[2]) for w in work)
 
 
+class _KernelNode(C.Structure):
+    """CUDA_KERNEL_NODE_PARAMS (v2) of the driver's API."""
+
+    _fields_ = [("func", C.c_void_p), ("grid", C.c_uint * 3), ("block", C.c_uint * 3), ("shared", C.c_uint),
+                ("params", C.c_void_p), ("extra", C.c_void_p), ("kern", C.c_void_p), ("ctx", C.c_void_p)]
+
+
+def launches(call):
+    """(cluster size, shared memory of a block) of the kernels that a call
+    launches, read from a captured graph."""
+    cu = C.CDLL("libcuda.so.1")
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    raw, n, found = C.c_void_p(graph.raw_cuda_graph()), C.c_size_t(), []
+    assert cu.cuGraphGetNodes(raw, None, C.byref(n)) == 0
+    nodes = (C.c_void_p * n.value)()
+    assert cu.cuGraphGetNodes(raw, nodes, C.byref(n)) == 0
+    for node in map(C.c_void_p, nodes):
+        kind, p, cluster, static = C.c_int(), _KernelNode(), (C.c_uint * 16)(), C.c_int()
+        assert cu.cuGraphNodeGetType(node, C.byref(kind)) == 0
+        if kind.value:     # CU_GRAPH_NODE_TYPE_KERNEL is 0
+            continue
+        assert cu.cuGraphKernelNodeGetParams_v2(node, C.byref(p)) == 0
+        assert cu.cuGraphKernelNodeGetAttribute(node, 4, cluster) == 0      # CU_LAUNCH_ATTRIBUTE_CLUSTER_DIMENSION
+        if p.func:         # CU_FUNC_ATTRIBUTE_SHARED_SIZE_BYTES
+            assert cu.cuFuncGetAttribute(C.byref(static), 1, C.c_void_p(p.func)) == 0
+        else:
+            assert cu.cuKernelGetAttribute(C.byref(static), 1, C.c_void_p(p.kern), 0) == 0
+        found.append((max(cluster[0], 1), p.shared + static.value))
+    return found
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,size", [(16, 600, 4096, 0), (64, 200, 8192, 0), (1024, 20000, 64, 2), (600, 30000, 200, 2),
+                                        (24, 32001, 1024, 1), (100, 300, 64, 1)])
+def test_clusters_have_their_multiprocessors_to_themselves(m, n, k, size):
+    """Blocks of a cluster need tensor memory all at once, so no block that might
+    hold some, of whatever kernel, may lie beside them: their shared memory
+    leaves less than the 1024 bytes that every block is charged."""
+    a, sa = i8(m, k, 1)
+    b, sb = i8(n, k, 2)
+    matmul_i8(a, sa, b, sb)
+    (cluster, shared), = launches(lambda: matmul_i8(a, sa, b, sb))
+    assert cluster == size or (size == 0 and cluster > 1)      # 0: split along k
+    whole = torch.cuda.get_device_properties(0).shared_memory_per_multiprocessor
+    assert cluster == 1 or 0 <= whole - 1024 - shared < 1024
+
+
 @pytest.mark.gpu
 def test_streams_and_graphs():
     x = torch.randn(50, 200, device="cuda")
