@@ -47,6 +47,8 @@ int dev_upload(T*& dst, const T* src, size_t count, int64_t& bytes) {
 }
 
 // Runs `launch(sm_count)` with `device` current and puts the caller's device back.
+// The thread's last error is cleared before (a refused allocation of an earlier
+// call would be taken for this launch's) and after a failure.
 template <typename F>
 int run_on_device(const char* who, int32_t device, F&& launch) {
   int ndev = 0;
@@ -56,7 +58,9 @@ int run_on_device(const char* who, int32_t device, F&& launch) {
   GANN_CUDA(cudaGetDevice(&prev));
   if (prev != device) GANN_CUDA(cudaSetDevice(device));
   cudaError_t e = cudaDeviceGetAttribute(&sm, cudaDevAttrMultiProcessorCount, device);
+  cudaGetLastError();
   if (e == cudaSuccess) e = launch(sm);
+  if (e != cudaSuccess) cudaGetLastError();
   if (prev != device) cudaSetDevice(prev);
   if (e != cudaSuccess)
     return set_error(e == cudaErrorMemoryAllocation ? GANN_ENOMEM : GANN_ECUDA,

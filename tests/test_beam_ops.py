@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+from conftest import get_index
 from gustann_b200 import api
 from gustann_b200.api import GustANNError, beam_select, matmul_i8, quantize_rows, reorder_states
 
@@ -474,6 +475,28 @@ def test_codes_by_beam_search_over_codebooks():
     got = encode(beam_select, reorder_states, product)
     want = encode(plain_select, lambda st, p: [ref_reorder(s, p) for s in st], plain_product)
     assert torch.equal(got[1], want[1]) and torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
+
+
+@pytest.mark.gpu
+def test_calls_after_another_calls_refused_allocation(index_root):
+    """A call that ran out of memory leaves an error with the host thread, which
+    is not the next call's."""
+    info = get_index(index_root, "u8")
+    p = info["paths"]
+    g = api.GustANN(info["dtype"])
+    g.init_pure_mem(api.GustANNConfig(p["index_file"], p["pq_file_prefix"], p["nav_graph_prefix"]), True)
+    one = np.zeros(1, np.float32)
+    x = torch.randn(8, 64, device="cuda")
+    sc, lg = make(2, 3, 300, "f32", 0)
+    c, s = quantize_rows(x)
+    par = torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    for call in (lambda: quantize_rows(x), lambda: matmul_i8(c, s, c, s), lambda: matmul_i8(c[:1], s[:1], c, s),
+                 lambda: beam_select(sc, lg, 4), lambda: beam_select(sc, lg, 4, log_softmax=True),
+                 lambda: reorder_states(lg, par)):
+        # 2^40 queries: refused before any is read
+        assert api.lib.gann_probe_lut(g._h, one.ctypes.data, 2 ** 40, one.ctypes.data) == api.GANN_ENOMEM
+        call()
+    g.close()
 
 
 # ------------------------------------------------------------------ refusals
