@@ -711,7 +711,7 @@ def reorder_states(states, parents, out=None, stream: int | None = None):
         _check_targets(srcs, dsts, parents, g, k)
     if stream is not None:
         with _stream_scope(dev, stream):
-            return reorder_states(states, parents, out)
+            return reorder_states(srcs[0] if one else srcs, parents, None if out is None else dsts)
     if out is None:
         dsts = [torch.empty(g, k, *s.shape[2:], dtype=s.dtype, device=dev) for s in srcs]
     table = []

@@ -385,6 +385,26 @@ def test_reorder_parents_that_are_no_beams():
 
 
 @pytest.mark.gpu
+def test_reorder_takes_any_iterable():
+    """States and targets may come from generators, on a given stream too."""
+    states = states_of(3, 4, 1)
+    p = torch.randint(0, 4, (3, 4), device="cuda", dtype=torch.int32)
+    want = [ref_reorder(s, p) for s in states]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for stream in (None, 0, side.cuda_stream):
+        new = reorder_states((s for s in states), p, stream=stream)
+        outs = [torch.zeros_like(w) for w in want]
+        torch.cuda.synchronize()
+        into = reorder_states((s for s in states), p, out=(o for o in outs), stream=stream)
+        one = reorder_states(states[0], p, stream=stream)
+        torch.cuda.synchronize()
+        assert len(new) == len(into) == len(want) and torch.equal(one, want[0])
+        for a, b, o, w in zip(new, into, outs, want):
+            assert torch.equal(a, w) and torch.equal(b, w) and torch.equal(o, w)
+
+
+@pytest.mark.gpu
 def test_reorder_many_states_and_many_groups():
     g = 70000
     s = torch.randint(0, 99, (g, 2, 3), device="cuda", dtype=torch.int16)
