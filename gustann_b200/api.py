@@ -738,18 +738,22 @@ def _check_targets(srcs, dsts, parents, g, k):
             _fail("reorder_states: a target must be [g, k, ...] of its state's type, or the state itself")
         if same and k > s.shape[1]:
             _fail("reorder_states: in place needs k <= w")
-        if not _apart(d):
+        # in place a group's rows are read before any is written, so no other
+        # group's may lie among them, in beams that are only read neither
+        if not _apart(d) or (d.data_ptr() == s.data_ptr() and not _apart(s)):
             _fail("reorder_states: elements of a target share memory")
     # every target apart from every other array, but for its own state in place
     spans = sorted([(*_extent(d), i, True) for i, d in enumerate(dsts)] +
-                   [(*_extent(s), i, False) for i, s in enumerate(srcs) if s.data_ptr() != dsts[i].data_ptr()] +
-                   [(*_extent(parents), -1, False)])
-    end, end_target = 0, 0
-    for a, b, _, target in spans:
-        if a < (end if target else end_target) and b > a:
-            _fail("reorder_states: a target overlaps another array")
-        end = max(end, b)
-        end_target = max(end_target, b if target else 0)
+                   [(*_extent(s), i, False) for i, s in enumerate(srcs)] + [(*_extent(parents), -1, False)])
+    before = []   # those that end behind the start of the present one
+    for a, b, i, target in spans:
+        before = [x for x in before if x[0] > a] if b > a else before
+        for _, j, other in before if b > a else ():
+            own = i == j and dsts[i].data_ptr() == srcs[i].data_ptr()
+            if (target or other) and not own:
+                _fail("reorder_states: a target overlaps another array")
+        if b > a:
+            before.append((b, i, target))
 
 
 def pivot_sample(n: int, s: int, seed: int = 114514) -> np.ndarray:

@@ -584,6 +584,26 @@ def test_state_layouts():
     assert api._extent(t) == (t.data_ptr(), t.data_ptr() + 4 * t.numel())
 
 
+def targets(monkeypatch, srcs, dsts, k):
+    """The check of targets, on tensors of the host."""
+    monkeypatch.setattr(api, "_on_cuda", lambda who, *t: (t[0].device, 0))
+    g = srcs[0].shape[0]
+    api._check_targets(srcs, dsts, torch.zeros(g, k, dtype=torch.int32), g, k)
+
+
+def test_targets_that_lie_among_beams_that_are_only_read(monkeypatch):
+    # groups that share beams: what one writes another reads
+    s = torch.zeros(64).as_strided((2, 4, 8), (16, 8, 1))
+    rejects(targets, monkeypatch, [s], [s[:, :2]], 2)
+    rejects(targets, monkeypatch, [s], [s], 4)
+    # one state's target in another's beams behind its own target
+    x = torch.zeros(1, 5, 8)
+    rejects(targets, monkeypatch, [x, torch.zeros(1, 5, 8)], [x[:, :2], x[:, 3:]], 2)
+    targets(monkeypatch, [x, torch.zeros(1, 5, 8)], [x[:, :2], torch.zeros(1, 2, 8)], 2)
+    targets(monkeypatch, [x], [x], 5)
+    targets(monkeypatch, [x, x], [torch.zeros(1, 2, 8), torch.zeros(1, 2, 8)], 2)
+
+
 @pytest.mark.gpu
 def test_refusals_on_the_gpu():
     sc, lg = make(2, 3, 8, "f32", 1)
