@@ -502,8 +502,35 @@ def _extent(t):
 
 
 def _disjoint(a, b) -> bool:
+    """Two tensors share no memory (sufficient test): one lies behind the other,
+    or they lie side by side in every period of their strides, largest first, as
+    slices of one array do."""
     (a0, a1), (b0, b1) = _extent(a), _extent(b)
-    return a1 <= b0 or b1 <= a0
+    if a1 <= b0 or b1 <= a0 or a0 == a1 or b0 == b1:
+        return True
+    if a0 > b0:
+        a, b, a0, b0 = b, a, b0, a0
+    gap = b0 - a0     # from a's start to b's, within the period
+    left = sorted(((s * a.element_size(), n) for n, s in zip(a.shape, a.stride()) if n > 1), reverse=True)
+    right = sorted(((s * b.element_size(), n) for n, s in zip(b.shape, b.stride()) if n > 1), reverse=True)
+    la, lb = a.element_size(), b.element_size()     # bytes of one element
+    while left or right:
+        period = max(d[0][0] for d in (left, right) if d)
+        if period == 0:
+            return False
+        for d in (left, right):   # a tensor without this stride has one period
+            if d and d[0][0] == period:
+                d.pop(0)
+        gap %= period
+        wa, wb = (sum((n - 1) * s for s, n in d) + e for d, e in ((left, la), (right, lb)))
+        if gap + wb > period:     # count from b's start instead
+            gap = (period - gap) % period
+            left, right, la, lb, wa, wb = right, left, lb, la, wb, wa
+        if wa > period or gap + wb > period:
+            return False
+        if gap >= wa:
+            return True
+    return False
 
 
 def quantize_rows(x, stream: int | None = None):
@@ -692,7 +719,8 @@ def reorder_states(states, parents, out=None, stream: int | None = None):
     :func:`beam_select` returns; a parent outside [0, w) gives zeros. Without
     ``out`` new tensors [g, k, ...] are returned; ``out`` gives the targets,
     and may be ``states`` itself: in place (k <= w; beams from k on stay as they were).
-    Other overlaps are refused. ``stream`` as in :func:`quantize_rows`."""
+    Slices of one array (keys and values) may be states and targets side by
+    side; other overlaps are refused. ``stream`` as in :func:`quantize_rows`."""
     torch = _get_torch()
     one = torch.is_tensor(states)
     srcs = [states] if one else list(states)
@@ -747,13 +775,15 @@ def _check_targets(srcs, dsts, parents, g, k):
                    [(*_extent(s), i, False) for i, s in enumerate(srcs)] + [(*_extent(parents), -1, False)])
     before = []   # those that end behind the start of the present one
     for a, b, i, target in spans:
-        before = [x for x in before if x[0] > a] if b > a else before
-        for _, j, other in before if b > a else ():
+        if b == a:
+            continue
+        t = parents if i < 0 else dsts[i] if target else srcs[i]
+        before = [x for x in before if x[0] > a]
+        for _, j, other, u in before:
             own = i == j and dsts[i].data_ptr() == srcs[i].data_ptr()
-            if (target or other) and not own:
+            if (target or other) and not own and not _disjoint(t, u):
                 _fail("reorder_states: a target overlaps another array")
-        if b > a:
-            before.append((b, i, target))
+        before.append((b, i, target, t))
 
 
 def pivot_sample(n: int, s: int, seed: int = 114514) -> np.ndarray:

@@ -604,6 +604,63 @@ def test_targets_that_lie_among_beams_that_are_only_read(monkeypatch):
     targets(monkeypatch, [x, x], [torch.zeros(1, 2, 8), torch.zeros(1, 2, 8)], 2)
 
 
+def test_targets_side_by_side_in_one_array(monkeypatch):
+    kv = torch.zeros(2, 3, 2, 4, 5)          # keys and values of one array
+    both = [kv[:, :, 0], kv[:, :, 1]]
+    targets(monkeypatch, both, both, 3)
+    rows = torch.zeros(2, 3, 24)             # parts of each row, of different widths
+    parts = [rows[..., :10], rows[..., 10:11], rows[..., 11:]]
+    targets(monkeypatch, parts, parts, 3)
+    targets(monkeypatch, [kv[:, :, 0]], [kv[:, :, 1]], 3)
+    rejects(targets, monkeypatch, [rows[..., :10], rows[..., 9:]], [rows[..., :10], rows[..., 9:]], 3)
+    rejects(targets, monkeypatch, [kv[:, :, 0], kv[:, :, 0, 1:]], [kv[:, :, 0], kv[:, :, 0, 1:]], 3)
+    rejects(targets, monkeypatch, [kv[..., 1:4]], [kv[..., 2:]], 3)
+
+
+def test_disjoint_against_every_address():
+    """Never true of tensors that share an element, and true of slices side by side."""
+    gen = np.random.default_rng(0)
+    buf = torch.zeros(4096, dtype=torch.uint8)
+    kept = {torch.uint8: buf, torch.int16: buf.view(torch.int16), torch.float32: buf.view(torch.float32)}
+    apart = shared = found = 0
+    for _ in range(6000):
+        two = []
+        strides = [int(gen.integers(1, 6)), int(gen.integers(1, 25)), int(gen.integers(1, 90))]
+        for dt in [list(kept)[int(gen.integers(3))]] * 2 if gen.random() < 0.8 else [torch.uint8, torch.float32]:
+            shape = [int(gen.integers(1, 5)) for _ in strides]
+            st = strides if gen.random() < 0.8 else [int(x) for x in gen.permutation(strides)]
+            two.append(kept[dt].as_strided(shape, st, int(gen.integers(0, 150))))
+        used = []
+        for t in two:
+            at = torch.zeros(1, dtype=torch.int64)
+            for n, st in zip(t.shape, t.stride()):
+                at = (at[:, None] + torch.arange(n) * st).flatten()
+            first = t.storage_offset() * t.element_size()
+            used.append({first + x * t.element_size() + e for x in at.tolist() for e in range(t.element_size())})
+        meet = bool(used[0] & used[1])
+        said = api._disjoint(*two)
+        assert said == api._disjoint(*reversed(two)) or not meet
+        assert not (said and meet)
+        apart, shared, found = apart + (not meet), shared + meet, found + said
+    assert shared > 1000 and apart > 1000 and found > apart // 2
+    for a, b in ((buf[:4000].view(10, 20, 20)[:, :, :7], buf[:4000].view(10, 20, 20)[:, :, 7:]),
+                 (buf[5:4005].view(10, 20, 20)[1:, :, :7], buf[:4000].view(10, 20, 20)[:, :, 0:5])):
+        assert api._disjoint(a, b) and api._disjoint(b, a)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [1, 3, 4])
+def test_reorder_slices_of_one_array_in_place(k):
+    g, w = 5, 4
+    kv = torch.randn(g, w, 3, 2, 7, 6, device="cuda")       # layers, keys and values, positions
+    before = kv.clone()
+    states = [kv[:, :, layer, i, :5] for layer in range(3) for i in range(2)]
+    p = torch.randint(-1, w, (g, k), device="cuda", dtype=torch.int32)
+    reorder_states(states, p, out=[s[:, :k] for s in states] if k < w else states)
+    assert torch.equal(kv[:, :k, :, :, :5], ref_reorder(before[:, :, :, :, :5], p))
+    assert torch.equal(kv[:, k:], before[:, k:]) and torch.equal(kv[:, :, :, :, 5:], before[:, :, :, :, 5:])
+
+
 @pytest.mark.gpu
 def test_refusals_on_the_gpu():
     sc, lg = make(2, 3, 8, "f32", 1)
