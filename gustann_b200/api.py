@@ -741,6 +741,8 @@ def reorder_states(states, parents, out=None, stream: int | None = None):
         with _stream_scope(dev, stream):
             return reorder_states(srcs[0] if one else srcs, parents, None if out is None else dsts)
     if out is None:
+        # the memory of a conjugate or negative view holds other values
+        srcs = [s.resolve_conj().resolve_neg() for s in srcs]
         dsts = [torch.empty(g, k, *s.shape[2:], dtype=s.dtype, device=dev) for s in srcs]
     table = []
     for s, d in zip(srcs, dsts):
@@ -764,6 +766,8 @@ def _check_targets(srcs, dsts, parents, g, k):
         same = d.data_ptr() == s.data_ptr() and d.shape == s.shape and d.stride() == s.stride()
         if d.dtype != s.dtype or d.shape != ((g,) + (s.shape[1] if same else k,) + s.shape[2:]):
             _fail("reorder_states: a target must be [g, k, ...] of its state's type, or the state itself")
+        if d.is_conj() != s.is_conj() or d.is_neg() != s.is_neg():
+            _fail("reorder_states: a state and its target must both be conjugate (or negative) views or neither")
         if same and k > s.shape[1]:
             _fail("reorder_states: in place needs k <= w")
         # in place a group's rows are read before any is written, so no other

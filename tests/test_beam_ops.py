@@ -405,6 +405,20 @@ def test_reorder_takes_any_iterable():
 
 
 @pytest.mark.gpu
+def test_reorder_conjugate_views():
+    z = torch.randn(3, 4, 5, dtype=torch.complex64, device="cuda")
+    p = torch.randint(-1, 4, (3, 4), device="cuda", dtype=torch.int32)
+    for s in (z, z.conj(), z.conj().imag, z.imag):
+        got = reorder_states(s, p)
+        assert torch.equal(got, ref_reorder(s, p))
+    rejects(reorder_states, z.conj(), p, out=torch.zeros_like(z))
+    rejects(reorder_states, z.conj().imag, p, out=torch.zeros(3, 4, 5, device="cuda"))
+    into = torch.zeros_like(z)
+    reorder_states(z.conj(), p, out=into.conj())
+    assert torch.equal(into.conj(), ref_reorder(z.conj(), p))
+
+
+@pytest.mark.gpu
 def test_reorder_many_states_and_many_groups():
     g = 70000
     s = torch.randint(0, 99, (g, 2, 3), device="cuda", dtype=torch.int16)
