@@ -587,7 +587,9 @@ def matmul_i8(a, a_scales, b, b_scales, bias=None, dtype=None, out=None, stream:
     Returns ``out`` [m, n] of ``dtype`` (float32 unless given; float16 and
     bfloat16 too), or fills ``out`` when it is given (contiguous rows).
     Queries against base rows: their scores; tokens against the rows of a
-    weight matrix: a linear layer. ``stream`` as in :func:`quantize_rows`."""
+    weight matrix: a linear layer. A GPU that does not serve the kernel for
+    about 4 s leaves NaN in what it has not made. ``stream`` as in
+    :func:`quantize_rows`."""
     torch = _get_torch()
     m, k, sa = _i8_rows("a", a, a_scales)
     n, kb, sb = _i8_rows("b", b, b_scales)

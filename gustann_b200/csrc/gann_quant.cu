@@ -35,7 +35,9 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) {
   return __float2bfloat16_rn(x);
 }
 
-// The scale of a row and what its entries are multiplied by. A tiny scale
+// The scale of a row and what its entries are multiplied by. The maximum times
+// 1/127 in float32 is off by 0.56 of a step at most (the quotient would be by
+// 0.5); the codes refer to the scale as it is stored. A tiny scale
 // (its reciprocal could overflow) is worked with 2^64 times larger, which
 // changes no quotient.
 struct RowScale {
@@ -114,7 +116,10 @@ __device__ __forceinline__ uint32_t quant_word(float x0, float x1, float x2, flo
 // element, and the codes take about seven instructions each. The row's 16-byte
 // vectors (VEC: rows start on 16-byte boundaries) stay in registers between
 // the maximum and the codes, up to kRowHeld a thread; longer rows are read
-// again, which the caches serve. 500000 x 768 f32: 328 us, 5.9 TB/s.
+// again, which the caches serve. 500000 x 768 f32: 305 to 330 us (5.8 TB/s and
+// more), bf16 298 us (3.9 TB/s: the instructions of a code are the same). Rows off
+// 16-byte boundaries are read element by element, and twice: 500000 x 769 f32 459
+// us, bf16 458. Rows of zeros take the codes' exact form: 442 us.
 constexpr int kRowHeld = 8;
 
 template <typename T, bool VEC, int WARPS>
@@ -207,8 +212,8 @@ __device__ __forceinline__ float i8_value(int acc, float sa, float sb, float bia
 // keeps up with it. A group of `lanes` lanes (as few as its vectors of 16 codes
 // need, at least 8) takes R rows of b at a time, so a's vector is read from
 // shared memory once for R of b's and R loads are on their way; the R sums are
-// folded into the lanes while they are added up. 1 x 100000 x 768: 13 to 14 us
-// (5.5 TB/s and more), on the tensor cores 21.6 us.
+// folded into the lanes while they are added up. 1 x 100000 x 768: 14 us (5.4
+// TB/s), on the tensor cores 21.6 us.
 constexpr int kThinRows = 4, kThinThreads = 256, kThinBytes = 48 * 1024;
 
 __device__ __forceinline__ int dot16(const uint4& x, const uint4& y, int acc) {
@@ -324,8 +329,9 @@ __global__ void __launch_bounds__(kThinThreads) thin_kernel(const int8_t* __rest
 // through distributed shared memory (integers: the order does not matter).
 //
 // Measured: 8192^3 395 us (2.8 PFLOP/s; the power limit holds the tensor pipe
-// there), 4097 x 4096 x 4096 to bf16 58 us, 4096 x 131072 x 768 to f32 500 us
-// (the output alone is 330 us of writes), 24 x 32001 x 1024 12 us.
+// there), 4097 x 4096 x 4096 to bf16 57 to 68 us, 4096 x 131072 x 768 to f32 500
+// us alone and up to 600 in a long run at the power limit (the output is 330 us
+// of writes; the epilogue stores 4 bytes a lane), 24 x 32001 x 1024 11 us.
 //
 // Waits for copies, products and buffers end: after kWaitClocks the block gives
 // up, and the tiles it has not finished are filled with NaN (there is no other

@@ -309,9 +309,14 @@ struct Held {
 //     Listed is same_sum(x), so that the order is that of the 64-bit sums with
 //     the score; the threshold lies at or below every x of an equal sum.
 // A segment writes its `keep` best and its sum; merge_kernel joins them.
-// Bound by instructions: 64 x 4 x 128000 bf16 with log-softmax takes 34 us with
-// its join (1.9 TB/s; reading alone would be 10), about 14 warp instructions an
-// element, of which the exponential, its argument and sum are four.
+// 64 x 4 x 128000 bf16 with log-softmax takes 36 us with its join (reading alone
+// would be 10): 25 us here, where 14 warp instructions for 32 elements (the
+// exponential, its argument and sum are four of them) issue in 55 % of the slots:
+// 16 warps an SM wait for their own last results, hardly for loads. The join
+// takes 10 us.
+// Where most elements pass the threshold they are listed one a lane a round:
+// equal rows of that size take 139 us, rows masked but for four tokens by the
+// type's lowest value 146 (by -inf 28), ascending rows 227.
 constexpr int kRowWarps = 4, kRowVecs = 4;
 constexpr int kRowTile = kRowVecs * kWarp;   // vectors
 
@@ -504,9 +509,11 @@ __global__ void __launch_bounds__(kRowWarps* kWarp, 4) row_kernel(const T* __res
 // passes are read again (from L1), one a lane at a time, and their elements at
 // or above the threshold are listed as (f, index); the sort by that is looked
 // over for equal f, which are put in the order of their 64-bit values.
-// 100000 x 8 x 256 f32, keep 8: 182 us (4.6 TB/s), bound by instructions and
-// the latency of one tile a warp; 10000 x 8 x 100, keep 100: 52 us, most of it
-// the sort of 128.
+// 100000 x 8 x 256 f32, keep 8: 182 us (4.6 TB/s; 17 warp instructions for 32
+// elements would be 97), bound by the latency of one tile a warp, which is
+// loaded, waited for and worked through; 10000 x 8 x 100, keep 100: 51 us, most
+// of it the sort of 128. Groups of equal entries take 1260 us at the first size,
+// four entries left 760 (the rest -inf) or 1110 (the type's lowest value).
 constexpr int kGroupWarps = 4;
 
 template <typename T, int VW>
@@ -946,7 +953,9 @@ namespace {
 // GPU holds at a time, and joined by a second kernel. Sixteen warps an SM: more
 // warps leave each fewer tiles to pay for its threshold with and the join more
 // candidates (64 x 4 x 128000 bf16, keep 8: 34 us with 16, 35 with 20, 38 with
-// 24, 45 with 32).
+// 24, 45 with 32, before the segments compared 64-bit sums, which costs under a
+// microsecond). The number of SMs is a constant because the workspace's size
+// follows from it, and that is asked for without a device.
 constexpr int kResidentWarps = 148 * 16;
 constexpr int kSmallGroup = 4096, kLargeGroup = 65536;   // bytes of a group
 
@@ -1027,8 +1036,8 @@ cudaError_t run_split(const SelectArgs& a, const SelectPlan& p, int sm_count, cu
                         : many    ? run(row_kernel<T, false, true>)
                                   : run(row_kernel<T, false, false>);
   if (e != cudaSuccess) return e;
-  // the join may be set up while the last segments still run; it waits for
-  // them itself
+  // the join's launch is prepared while the segments run; its blocks start when
+  // the last of theirs has ended, since none of them lets it start sooner
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;

@@ -393,7 +393,9 @@ int gann_quantize_rows(const void* d_x, int64_t rows, int64_t x_stride, int32_t 
  *   out        [m x out_stride elements] of out_dtype (gann_float),
  *              out_stride >= n; elements of a row past n are left as they were
  * Device buffers on `device`, enqueued on `stream`; the output may not overlap
- * an input. 1 <= k <= 131071; m, n < 2^31. No allocation. */
+ * an input. 1 <= k <= 131071; m, n < 2^31. No allocation. Should the GPU's copies
+ * or products not come within about 4 s, the kernel ends and the parts of the
+ * output that it had not made hold NaN; there is no other sign of it. */
 int gann_matmul_i8(const int8_t* d_a, int64_t m, int64_t a_stride, const float* d_a_scales, const int8_t* d_b,
                    int64_t n, int64_t b_stride, const float* d_b_scales, const float* d_bias, int32_t k, void* d_out,
                    int64_t out_stride, int32_t out_dtype, int32_t device, void* stream);
@@ -406,8 +408,8 @@ int gann_matmul_i8(const int8_t* d_a, int64_t m, int64_t a_stride, const float* 
  * and the candidates are ordered by that value, largest first, compared in 64
  * bits, equal ones by b * vocab + t. (Pass negated distances.) With log_softmax
  * the sum of the exponentials is gathered in float32 and joined in 64 bits, so
- * the values of one beam share an error of less than 2^-17 (about 1e-7 as a
- * rule), and candidates of different beams nearer than that to each other may
+ * the values of one beam share an error of less than 2^-17 (at most 4e-7
+ * measured), and candidates of different beams nearer than that to each other may
  * trade places; a beam's own candidates are ordered by scores + logits in 64
  * bits, equal ones by t.
  *   logits    [groups][beams][vocab] of dtype (gann_float); strides in elements
